@@ -74,6 +74,52 @@ class ChannelDeltaArgs(C.Structure):
                 + [(n, _SZ) for n in ("heads", "kv_heads", "dim", "vdim")] + [("eps", C.c_float)])
 
 
+# enum cg_rotation_scaling
+ROTATION_PLAIN, ROTATION_LINEAR, ROTATION_BANDS, ROTATION_RAMP = range(4)
+
+
+# cg_rotation, cg_rotary_args, cg_cache_append_args, cg_cache_attention_args, cg_token_batch, cg_cache8, cg_rotary_rows, cg_cache_append_rows,
+# cg_cache_attention_rows
+class Rotation(C.Structure):
+    _fields_ = [("dims", _SZ), ("interleaved", _I), ("scaling", _I)] + [(n, C.c_double) for n in ("base", "factor", "low", "high", "original", "magnitude")]
+
+
+class RotaryArgs(C.Structure):
+    _fields_ = [("q", _P), ("k", _P)] + [(n, _SZ) for n in ("heads", "kv_heads", "dim", "position")] + [("rotation", Rotation)]
+
+
+class CacheAppendArgs(C.Structure):
+    _fields_ = [(n, _P) for n in ("k", "v", "k_codes", "v_codes", "k_scale", "v_scale")] + [("position", _SZ)]
+
+
+class CacheAttentionArgs(C.Structure):
+    _fields_ = ([(n, _P) for n in ("q", "k_codes", "v_codes", "k_scale", "v_scale")] + [(n, _SZ) for n in ("heads", "position", "window")]
+                + [("scale", C.c_float)])
+
+
+class TokenBatch(C.Structure):
+    _fields_ = [(n, _SZ) for n in ("sequences", "tokens", "position")] + [("held", _P), ("counts", _P)]
+
+
+class Cache8(C.Structure):
+    _fields_ = [(n, _P) for n in ("k_codes", "v_codes", "k_scale", "v_scale")] + [(n, _SZ) for n in ("kv_heads", "dim", "vdim", "capacity", "block")]
+
+
+class RotaryRows(C.Structure):
+    _fields_ = ([("batch", TokenBatch), ("dtype", _I)] + [(n, _P) for n in ("q", "k", "q_out", "k_out")]
+                + [(n, _SZ) for n in ("q_pitch", "k_pitch", "q_out_pitch", "k_out_pitch", "heads", "kv_heads", "dim", "rot_dims")]
+                + [("interleaved", _I), ("magnitude", C.c_float), ("turns", _P)])
+
+
+class CacheAppendRows(C.Structure):
+    _fields_ = [("batch", TokenBatch), ("dtype", _I), ("k", _P), ("v", _P), ("k_pitch", _SZ), ("v_pitch", _SZ), ("cache", Cache8)]
+
+
+class CacheAttentionRows(C.Structure):
+    _fields_ = ([("batch", TokenBatch), ("dtype", _I), ("q", _P), ("out", _P), ("q_pitch", _SZ), ("out_pitch", _SZ), ("heads", _SZ), ("cache", Cache8),
+                 ("scale", C.c_float), ("window", _SZ), ("workspace", _P), ("workspace_bytes", _SZ)])
+
+
 # name -> (restype, argtypes); every symbol the header declares.
 SIGNATURES = {
     "cg_backend_create": (_I, [_I, _PP]),
@@ -126,6 +172,14 @@ SIGNATURES = {
     "cg_block_token_side": (_I, [_P, C.POINTER(TokenSideArgs), _PP]),
     "cg_block_attention": (_I, [_P, C.POINTER(AttentionArgs), _PP, _PP, _PP]),
     "cg_block_channel_delta": (_I, [_P, C.POINTER(ChannelDeltaArgs), _PP, _PP, _PP]),
+    "cg_rotation_turns": (_I, [C.POINTER(Rotation), C.POINTER(C.c_double), C.POINTER(C.c_float)]),
+    "cg_block_rotary": (_I, [_P, C.POINTER(RotaryArgs), _PP, _PP]),
+    "cg_block_cache_append": (_I, [_P, C.POINTER(CacheAppendArgs), _PP, _PP, _PP, _PP]),
+    "cg_block_cache_attention": (_I, [_P, C.POINTER(CacheAttentionArgs), _PP]),
+    "cg_rotary_noalloc": (_I, [_I, C.POINTER(RotaryRows), _P]),
+    "cg_cache_append_noalloc": (_I, [_I, C.POINTER(CacheAppendRows), _P]),
+    "cg_cache_attention_workspace": (_I, [C.POINTER(CacheAttentionRows), _SZP]),
+    "cg_cache_attention_noalloc": (_I, [_I, C.POINTER(CacheAttentionRows), _P]),
 }
 
 

@@ -379,6 +379,40 @@ class Backend:
         """-> (output, state, convolution state)."""
         return self._three(self._lib.cg_block_channel_delta, self._block(A.ChannelDeltaArgs, tensors, options))
 
+    # ---- rotary positions and the 8-bit cache (their section of include/catgrad_hip.h) ---------
+    def rotation_turns(self, **rotation):
+        """-> (turns a position of each pair, as float64; magnitude); rotation: the fields of cg_rotation."""
+        r, m = A.Rotation(**rotation), C.c_float()
+        turns = np.zeros(max(r.dims // 2, 1), np.float64)
+        self._check(self._lib.cg_rotation_turns(C.byref(r), turns.ctypes.data_as(C.POINTER(C.c_double)), C.byref(m)))
+        return turns, float(m.value)
+
+    def block_rotary(self, q, k=None, rotation=None, **options):
+        """-> (q, k) turned (k: None where there is none); rotation: a dictionary with the fields of cg_rotation."""
+        a = self._block(A.RotaryArgs, dict(q=q, k=k), options)
+        a.rotation = A.Rotation(**(rotation or {}))
+        qo, ko = C.c_void_p(), C.c_void_p()
+        self._check(self._lib.cg_block_rotary(self._b, C.byref(a), C.byref(qo), C.byref(ko)))
+        return Tensor(self, qo.value), Tensor(self, ko.value) if ko.value else None
+
+    def empty_cache(self, sequences: int, kv_heads: int, dim: int, vdim: int, capacity: int, block: int = 64) -> dict:
+        """The tensors of an 8-bit cache with room for `capacity` positions (whole blocks)."""
+        n = capacity // block
+        return dict(k_codes=self.zeros((sequences, kv_heads, capacity, dim), A.F8), v_codes=self.zeros((sequences, kv_heads, n, vdim, block), A.F8),
+                    k_scale=self.zeros((sequences, kv_heads, n), A.F32), v_scale=self.zeros((sequences, kv_heads, n), A.F32))
+
+    def block_cache_append(self, k, v, cache: dict, position: int) -> dict:
+        """-> the cache (a dictionary as of `empty_cache`) with the new tokens' keys and values; in place where the tensors are
+        given up with `Tensor.move()` and nobody else holds them."""
+        a = self._block(A.CacheAppendArgs, dict(k=k, v=v, **cache), dict(position=position))
+        o = [C.c_void_p() for _ in range(4)]
+        self._check(self._lib.cg_block_cache_append(self._b, C.byref(a), *[C.byref(p) for p in o]))
+        return {n: Tensor(self, p.value) for n, p in zip(("k_codes", "v_codes", "k_scale", "v_scale"), o)}
+
+    def block_cache_attention(self, q, cache: dict, heads: int, position: int, scale: float, window: int = 0) -> Tensor:
+        a = self._block(A.CacheAttentionArgs, dict(q=q, **cache), dict(heads=heads, position=position, scale=scale, window=window))
+        return self._op(lambda b, o: self._lib.cg_block_cache_attention(b, C.byref(a), o))
+
 
 _hip_lib = None
 

@@ -1,0 +1,175 @@
+// New tokens' keys and values into the 8-bit cache (their section of include/catgrad_hip.h).
+//
+// A workgroup takes one block of positions of one head, of the keys or of the values, from the first new token that falls into it to
+// the last: the largest magnitude of what is new, the block's exponent e, the codes.  All new values are asked for at once and stay in
+// registers between the two, so they are read once.  Keys lie token by token: a thread takes 16 channels of a token.  Values lie channel by
+// channel: a thread takes 16 neighbouring positions of a channel, reads them from 16 rows (a wave's lanes take neighbouring
+// channels) and stores them in one piece, together with what the piece held of older positions.  No two workgroups share a byte
+// that either writes.  A block that grew has the rest of its codes rounded anew in a second sweep, which few appends need.
+#include "block_cache.hpp"
+#include "device_utils.hpp"
+
+#include <algorithm>
+
+namespace cg {
+namespace {
+
+constexpr uint32_t kThreads = 256, kPiece = 16; // bytes (codes) of a unit of work
+
+__device__ __forceinline__ float code_range(float x) { // within the codes' range; NaN stays
+    const float c = __builtin_amdgcn_fmed3f(x, -448.0f, 448.0f);
+    return x == x ? c : x;
+}
+__device__ __forceinline__ uint32_t codes_of(const float *x, float inv) { // the nearest codes (ties to even) to four values times inv
+    int c = __builtin_amdgcn_cvt_pk_fp8_f32(code_range(x[0] * inv), code_range(x[1] * inv), 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(code_range(x[2] * inv), code_range(x[3] * inv), c, true);
+}
+__device__ __forceinline__ uint32_t rounded_anew(uint32_t codes, float factor) {
+    const float x[4] = {__builtin_amdgcn_cvt_f32_fp8(codes, 0), __builtin_amdgcn_cvt_f32_fp8(codes, 1), __builtin_amdgcn_cvt_f32_fp8(codes, 2),
+                        __builtin_amdgcn_cvt_f32_fp8(codes, 3)};
+    return codes_of(x, factor);
+}
+__device__ __forceinline__ uint4 rounded_anew(uint4 c, float f) { return make_uint4(rounded_anew(c.x, f), rounded_anew(c.y, f), rounded_anew(c.z, f), rounded_anew(c.w, f)); }
+// The bytes of `mine` where take has ones, else those of `other`.
+__device__ __forceinline__ uint32_t either(uint32_t take, uint32_t mine, uint32_t other) { return (mine & take) | (other & ~take); }
+
+// The smallest e with size <= 448 * 2^e (448 = 1.75 * 2^8), within the limits.
+__device__ __forceinline__ int exponent_for(float size) {
+    const uint32_t u = __float_as_uint(size);
+    const int e = (int)(u >> 23) - 127 - 8 + ((u & 0x7FFFFFu) > 0x600000u ? 1 : 0);
+    return e < kLowestScale ? kLowestScale : e > kHighestScale ? kHighestScale : e;
+}
+__device__ __forceinline__ float largest_finite(float m, float x) { return fabsf(x) < INFINITY ? fmaxf(m, fabsf(x)) : m; }
+
+template <class T, int UNITS, bool VALUES> __device__ void append_block(const CacheAppendPlan &p, uint32_t b, uint32_t g, uint32_t nth, bool whole) {
+    __shared__ float sizes[kThreads / 64];
+    const Cache8 &c = p.cache;
+    const uint32_t n = 1u << c.block_log2, W = VALUES ? c.vdim : c.dim;
+    const uint64_t held = p.batch.held_by(b), j = (held >> c.block_log2) + nth, begin = j << c.block_log2;
+    if (begin >= c.capacity) return;
+    const uint64_t end = held + p.batch.count_of(b);
+    // new positions of the block, counted from its first
+    const uint32_t t0 = held > begin ? (uint32_t)(held - begin) : 0, t1 = (uint32_t)min((uint64_t)n, end > begin ? end - begin : 0);
+    if (t0 >= t1) return;
+    const uint64_t bg = (uint64_t)b * c.kv_heads + g, nb = c.capacity >> c.block_log2;
+    float *const scale = (VALUES ? c.v_scale : c.k_scale) + bg * nb + j;
+    const int had = t0 ? scale_exponent(*scale) : kLowestScale;
+    uint8_t *const codes = VALUES ? c.v_codes + (bg * nb + j) * W * n : c.k_codes + (bg * c.capacity + begin) * W;
+    // row 0: position `begin` (in front of the array where that is no new token: never addressed)
+    const int64_t pitch = VALUES ? p.v_pitch : p.k_pitch;
+    const T *const rows = static_cast<const T *>(VALUES ? p.v : p.k) + (int64_t)g * W;
+    const int64_t row0 = (int64_t)b * p.batch.tokens + (int64_t)begin - (int64_t)held;
+
+    const uint32_t first_piece = VALUES ? t0 / kPiece : 0, pieces = VALUES ? (t1 + kPiece - 1) / kPiece - first_piece : W / kPiece;
+    const uint32_t units = VALUES ? pieces * W : pieces * (t1 - t0);
+    float x[UNITS][kPiece];
+    uint4 old[UNITS];
+    uint4 *to[UNITS];
+    uint32_t piece[UNITS];
+    float size = 0.0f;
+#pragma unroll
+    for (int i = 0; i < UNITS; i++) {
+        const uint32_t id = i * kThreads + threadIdx.x;
+        to[i] = nullptr;
+        if (id >= units) continue;
+        if (VALUES) {
+            const uint32_t k = id / W, d = id - k * W;
+            piece[i] = (first_piece + k) * kPiece;
+            to[i] = reinterpret_cast<uint4 *>(codes + (uint64_t)d * n + piece[i]);
+            old[i] = *to[i];
+#pragma unroll
+            for (uint32_t q = 0; q < kPiece; q++) {
+                const uint32_t t = piece[i] + q;
+                x[i][q] = t >= t0 && t < t1 ? widened(rows[(row0 + t) * pitch + d]) : 0.0f;
+            }
+        } else {
+            const uint32_t t = id / pieces, k = id - t * pieces;
+            to[i] = reinterpret_cast<uint4 *>(codes + (uint64_t)(t0 + t) * W + k * kPiece);
+            load_elements<T, kPiece>(rows + (row0 + t0 + t) * pitch + k * kPiece, whole, x[i]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < UNITS; i++)
+        if (to[i])
+#pragma unroll
+            for (uint32_t q = 0; q < kPiece; q++) size = largest_finite(size, x[i][q]);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) size = fmaxf(size, __shfl_xor(size, o));
+    if (threadIdx.x % 64 == 0) sizes[threadIdx.x / 64] = size;
+    __syncthreads();
+    size = fmaxf(fmaxf(sizes[0], sizes[1]), fmaxf(sizes[2], sizes[3]));
+    const int e = max(had, exponent_for(size)); // (a size of 0: the lowest)
+    const bool grew = t0 && e > had;
+    const float inv = power_of_two(-e), down = power_of_two(max(had - e, -64)); // (2^-64 leaves nothing of any code)
+    if (threadIdx.x == 0) *scale = power_of_two(e); // (read by all in front of the barrier)
+#pragma unroll
+    for (int i = 0; i < UNITS; i++) {
+        if (!to[i]) continue;
+        uint4 r = make_uint4(codes_of(&x[i][0], inv), codes_of(&x[i][4], inv), codes_of(&x[i][8], inv), codes_of(&x[i][12], inv));
+        if (VALUES && (piece[i] < t0 || piece[i] + kPiece > t1)) {
+            const uint4 anew = grew ? rounded_anew(old[i], down) : old[i];
+            uint32_t m[4], past[4]; // bytes that are new, that are of older positions
+#pragma unroll
+            for (uint32_t w = 0; w < 4; w++) {
+                m[w] = past[w] = 0;
+#pragma unroll
+                for (uint32_t q = 0; q < 4; q++) {
+                    const uint32_t t = piece[i] + 4 * w + q;
+                    m[w] |= t >= t0 && t < t1 ? 255u << (8 * q) : 0;
+                    past[w] |= t < t0 ? 255u << (8 * q) : 0;
+                }
+            }
+            r = make_uint4(either(m[0], r.x, either(past[0], anew.x, old[i].x)), either(m[1], r.y, either(past[1], anew.y, old[i].y)),
+                           either(m[2], r.z, either(past[2], anew.z, old[i].z)), either(m[3], r.w, either(past[3], anew.w, old[i].w)));
+        }
+        *to[i] = r;
+    }
+    if (!grew) return;
+    // pieces that hold older positions alone
+    const uint32_t rest = VALUES ? t0 / kPiece * W : t0 * pieces;
+    for (uint32_t id = threadIdx.x; id < rest; id += kThreads) {
+        uint4 *at;
+        if (VALUES) {
+            const uint32_t k = id / W, d = id - k * W;
+            at = reinterpret_cast<uint4 *>(codes + (uint64_t)d * n + k * kPiece);
+        } else {
+            at = reinterpret_cast<uint4 *>(codes) + id;
+        }
+        *at = rounded_anew(*at, down);
+    }
+}
+
+template <class T, int UNITS> __global__ __launch_bounds__(kThreads) void cache_append_kernel(CacheAppendPlan p, uint32_t touched, bool k_whole) {
+    uint32_t id = blockIdx.x;
+    const uint32_t nth = id % touched;
+    id /= touched;
+    const bool values = id & 1;
+    id >>= 1;
+    const uint32_t g = id % p.cache.kv_heads, b = id / p.cache.kv_heads;
+    if (values) append_block<T, UNITS, true>(p, b, g, nth, false);
+    else append_block<T, UNITS, false>(p, b, g, nth, k_whole);
+}
+
+} // namespace
+
+int launch_cache_append(const LaunchOn &on, cg_dtype dtype, const CacheAppendPlan &p) {
+    const uint32_t n = 1u << p.cache.block_log2;
+    const uint32_t touched = std::min(p.cache.capacity / n, (p.batch.tokens + n - 2) / n + 1);
+    return with_element(dtype, [&](auto e) {
+        typedef decltype(e) T;
+        const bool whole = reinterpret_cast<uintptr_t>(p.k) % 16 == 0 && p.k_pitch * sizeof(T) % 16 == 0; // (dim is a multiple of 16)
+        const dim3 grid(touched * p.cache.kv_heads * p.batch.sequences * 2);
+        // what a thread keeps in registers: two pieces for blocks of up to 8192 codes, eight for the largest
+        return n * std::max(p.cache.dim, p.cache.vdim) <= 2 * kPiece * kThreads
+                   ? on("cache append launch", cache_append_kernel<T, 2>, grid, dim3(kThreads), p, touched, whole)
+                   : on("cache append launch", cache_append_kernel<T, 8>, grid, dim3(kThreads), p, touched, whole);
+    });
+}
+
+int load_cache_append_kernels() {
+    hipFuncAttributes a;
+    CG_HIP(hipFuncGetAttributes(&a, reinterpret_cast<const void *>(cache_append_kernel<float, 2>)));
+    return CG_OK;
+}
+
+} // namespace cg

@@ -1,0 +1,454 @@
+// Attention over the 8-bit cache (their section of include/catgrad_hip.h): the kernel, instantiated by element type in
+// block_cache_attention_{f32,f16,bf16}.hip and launched from block_cache_attention.hip.
+//
+// One pass over the codes with the running maximum and sum of the soft-max, on v_mfma_f32_16x16x32_f16.  A wave takes tiles of 64
+// positions and up to 32 rows (a row: one query head of one token; the heads that share a key / value head lie together), all in
+// registers.  The products are taken transposed, scores^T = K q^T and out^T = V^T P^T, with the positions of a tile dealt out so
+// that nothing has to change lanes between the two: the instruction leaves a lane four scores of one row (its column), at rows
+// 4 quad + i of the left operand, and wants eight neighbouring values of k of one column from it.  So row 4 a + i of the kt-th left
+// operand (kt = 0 .. 3) is position 16 a + 4 kt + i: a lane's 16 scores are the positions 16 quad .. 16 quad + 15 of its row, the
+// weights of the second product as they come, and its codes of a value channel for them are 16 neighbouring bytes (values lie
+// channel by channel within a block).  Channels of K are dealt out the same way, 16 neighbouring bytes of a position's key to a lane.  So all
+// codes come by 16-byte loads straight into the registers from which the instruction takes them, without LDS or barriers.
+//
+// Numbers.  E4M3 codes are exact in 16-bit floats.  A row of q is scaled by a power of two so that its largest magnitude lies
+// in [2^7, 2^8), and is one 16-bit float a value, or with 32-bit inputs the sum of two (2^-23 of the row's largest; 16-bit inputs are
+// exact but where they lie 2^22 below it).  A block's scale multiplies the scores in 32 bits.  Weights are exp2(score - m + 8) <= 2^15
+// with m the running maximum, which moves only where a score is 7 or more above it (most tiles move none: then nothing is
+// rescaled), as one 16-bit float (2^-12) or two (2^-23).  The second product of a tile starts from zero and is added to the
+// total by a vector instruction, with the value block's scale: the matrix instruction cuts its sums off, which over a long
+// cache would move all of them to one side, and the total is never in units of an earlier block's scale.  In blocks of 16 or 32 positions a tile's
+// scales differ: weights are multiplied by 2^(e - the largest e), and where those are more than 2^8 apart every block is a product of
+// its own.  The sum of weights is taken in 32 bits, of the weights before they are rounded.
+//
+// Positions that a row does not see: their weights are set to zero, and since zero times NaN is NaN, a tile that not all rows
+// see whole has its NaN codes of values taken out, and put back into the totals of the rows that do see them.
+#pragma once
+
+#include "block_cache.hpp"
+#include "device_utils.hpp"
+
+namespace cg {
+
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef _Float16 half8v __attribute__((ext_vector_type(8)));
+typedef float float4v __attribute__((ext_vector_type(4)));
+
+constexpr uint32_t kTile = 64;           // positions of a wave's tile
+constexpr uint32_t kWavesOfAttention = 4;
+constexpr float kNoMaximum = -3.0e38f;   // of a row that has seen nothing
+// The fewest tiles worth a part of their own, with the waves sharing a row's tiles and without.
+constexpr uint32_t kLeastTilesShared = 8, kLeastTilesRows = 8;
+
+// The positions that rows of the tokens s0 .. s1 of a sequence see, cut into at most `splits` parts of whole tiles.
+struct KeyRange {
+    uint32_t first_tile, end_tile, parts, each;
+};
+__device__ __forceinline__ KeyRange key_range(const CacheAttentionPlan &p, uint64_t held, uint32_t s0, uint32_t s1) {
+    const uint64_t C = p.cache.capacity, end = min(held + s1 + 1, C), q0 = held + s0 + 1;
+    const uint64_t lo = p.window && q0 > p.window ? min(q0 - p.window, end) : 0;
+    KeyRange r;
+    r.first_tile = (uint32_t)(lo / kTile);
+    r.end_tile = (uint32_t)((end + kTile - 1) / kTile);
+    const uint32_t n = r.end_tile - r.first_tile, least = p.rows_by_wave ? kLeastTilesRows : kLeastTilesShared;
+    r.parts = max(1u, min(p.splits, n / least));
+    r.each = (n + r.parts - 1) / r.parts;
+    return r;
+}
+
+#ifdef __HIPCC__
+// codes 2 i, 2 i + 1 of a word as 16-bit floats (exact)
+template <bool HIGH> __device__ __forceinline__ half2v two_of(uint32_t codes) { return __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)codes, 1.0f, HIGH); }
+__device__ __forceinline__ half8v eight_of(uint32_t lo, uint32_t hi) {
+    const half2v a = two_of<false>(lo), b = two_of<true>(lo), c = two_of<false>(hi), d = two_of<true>(hi);
+    return half8v{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+__device__ __forceinline__ uint32_t word_of(const uint4 &v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+// the k-th eight codes of sixteen
+__device__ __forceinline__ half8v eight_of(const uint4 &v, int k) { return eight_of(word_of(v, 2 * k), word_of(v, 2 * k + 1)); }
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t c) { return ((c & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u; } // bit 7 of the bytes that are NaN
+// over the four lanes that share a row
+__device__ __forceinline__ float quads_max(float x) {
+    x = fmaxf(x, __shfl_xor(x, 16));
+    return fmaxf(x, __shfl_xor(x, 32));
+}
+__device__ __forceinline__ int quads_max(int x) {
+    x = max(x, __shfl_xor(x, 16));
+    return max(x, __shfl_xor(x, 32));
+}
+__device__ __forceinline__ float quads_sum(float x) {
+    x += __shfl_xor(x, 16);
+    return x + __shfl_xor(x, 32);
+}
+
+// ROWS: every wave of a workgroup has rows of its own and walks all of their tiles; else the waves have the same rows, take the
+// tiles in turns and add their results up in LDS.  RT: 16-row groups of a wave.  NL: 64-channel pieces of a head.
+template <class T, int NL, int RT, bool ROWS>
+__global__ __launch_bounds__(64 * kWavesOfAttention, NL * RT > 2 ? 1 : 2) void cache_attention_kernel(CacheAttentionPlan p) {
+    constexpr int kPieces = sizeof(T) == 4 ? 2 : 1, NV = 4 * NL, kSteps = 2 * NL;
+    const Cache8 &c = p.cache;
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, quad = lane >> 4;
+    uint32_t id = blockIdx.x;
+    const uint32_t bg = id % p.bgs;
+    id /= p.bgs;
+    const uint32_t split = id % p.splits, row_block = p.row_blocks - 1 - id / p.splits; // (the longest rows first)
+    const uint32_t b = bg / c.kv_heads, g = bg - b * c.kv_heads;
+    const uint64_t held = p.batch.held_by(b);
+    const uint32_t R = p.batch.count_of(b) * p.rep, group = (ROWS ? kWavesOfAttention : 1) * 16 * RT, group0 = row_block * group;
+    if (group0 >= R) return;
+    const KeyRange range = key_range(p, held, group0 / p.rep, (min(group0 + group, R) - 1) / p.rep);
+    if (split >= range.parts) return;
+    uint32_t tile = range.first_tile + split * range.each, end_tile = min(tile + range.each, range.end_tile);
+    const uint32_t row0 = group0 + (ROWS ? wave * 16 * RT : 0);
+    if (ROWS) {
+        if (row0 >= R) return;
+        CacheAttentionPlan whole = p;
+        whole.splits = 1;
+        const KeyRange mine = key_range(whole, held, row0 / p.rep, (min(row0 + 16 * RT, R) - 1) / p.rep);
+        tile = max(tile, mine.first_tile);
+        end_tile = min(end_tile, mine.end_tile);
+    } else {
+        tile += wave;
+    }
+    constexpr uint32_t kStride = ROWS ? 1 : kWavesOfAttention;
+
+    // ---- the rows: their queries, and which positions they see
+    half8v q[RT][kPieces][kSteps];
+    float row_factor[RT];
+    int last[RT], begin[RT]; // positions begin .. last; none: last < begin
+    int64_t row_token[RT];   // (for the results)
+    const bool whole_q = reinterpret_cast<uintptr_t>(p.q) % 16 == 0 && p.q_pitch * sizeof(T) % 16 == 0;
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+        const uint32_t r = row0 + rt * 16 + col, rr = min(r, R - 1), s = rr / p.rep, head = g * p.rep + rr - s * p.rep;
+        row_token[rt] = (int64_t)b * p.batch.tokens + s;
+        const uint64_t at = held + s; // its position
+        last[rt] = r < R ? (int)min(at, (uint64_t)c.capacity - 1) : -1;
+        begin[rt] = p.window && at + 1 > p.window ? (int)min(at + 1 - p.window, (uint64_t)c.capacity) : 0;
+        const T *src = static_cast<const T *>(p.q) + row_token[rt] * p.q_pitch + head * c.dim;
+        float x[NL][16], size = 0.0f, bad = 0.0f;
+#pragma unroll
+        for (int l = 0; l < NL; l++) {
+            const uint32_t d = l * 64 + quad * 16;
+            if (d < c.dim) {
+                load_elements<T, 16>(src + d, whole_q, x[l]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; i++) x[l][i] = 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                size = fmaxf(size, fabsf(x[l][i]));
+                bad += x[l][i] * 0.0f;
+            }
+        }
+        size = quads_max(size);
+        bad = quads_sum(bad); // 0, or NaN where a value is not finite: then so are the row's scores
+        const int e = bad == 0.0f && size > 0.0f ? __builtin_amdgcn_frexp_expf(size) : 0;
+        row_factor[rt] = bad == 0.0f ? ldexpf(fabsf(p.scale) * 1.44269504088896341f, e - 8) : bad;
+        const float sign = p.scale < 0.0f ? -1.0f : 1.0f;
+#pragma unroll
+        for (int l = 0; l < NL; l++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const float y = bad == 0.0f ? ldexpf(x[l][i], 8 - e) * sign : 0.0f;
+                const _Float16 h = (_Float16)y;
+                q[rt][0][2 * l + i / 8][i % 8] = h;
+                if (kPieces == 2) q[rt][kPieces - 1][2 * l + i / 8][i % 8] = (_Float16)(y - (float)h);
+            }
+    }
+    // positions that all of the wave's rows see, and those that any does
+    int all_from = 0, all_to = 0x7FFFFFFF, any_from = 0x7FFFFFFF, any_to = -1;
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++)
+        if (last[rt] >= 0) {
+            all_from = max(all_from, begin[rt]);
+            all_to = min(all_to, last[rt]);
+            any_from = min(any_from, begin[rt]);
+            any_to = max(any_to, last[rt]);
+        }
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) {
+        all_from = max(all_from, __shfl_xor(all_from, o));
+        all_to = min(all_to, __shfl_xor(all_to, o));
+        any_from = min(any_from, __shfl_xor(any_from, o));
+        any_to = max(any_to, __shfl_xor(any_to, o));
+    }
+    all_from = __builtin_amdgcn_readfirstlane(all_from);
+    all_to = __builtin_amdgcn_readfirstlane(all_to);
+    any_from = __builtin_amdgcn_readfirstlane(any_from);
+    any_to = __builtin_amdgcn_readfirstlane(any_to);
+
+    // ---- the tiles
+    const uint32_t nb = c.capacity >> c.block_log2;
+    const uint8_t *const keys = c.k_codes + (uint64_t)bg * c.capacity * c.dim, *const values = c.v_codes + (uint64_t)bg * c.capacity * c.vdim;
+    const float *const k_scale = c.k_scale + (uint64_t)bg * nb, *const v_scale = c.v_scale + (uint64_t)bg * nb;
+    uint4 k_next[4][NL], k_now[4][NL], v_now[NV];
+    float ks_next = 0.0f, vs_next = 0.0f;
+    // (Addresses stay within the cache: a tile may reach behind its capacity, where no row sees anything.)
+    auto ask_keys = [&](uint32_t t) {
+#pragma unroll
+        for (int kt = 0; kt < 4; kt++) {
+            const uint32_t at = min(t * kTile + (col >> 2) * 16 + kt * 4 + (col & 3), c.capacity - 1);
+#pragma unroll
+            for (int l = 0; l < NL; l++) {
+                const uint32_t d = l * 64 + quad * 16; // behind dim the query is zero: any code of the same key will do
+                k_next[kt][l] = *reinterpret_cast<const uint4 *>(keys + (uint64_t)at * c.dim + (d < c.dim ? d : 0));
+            }
+        }
+        const uint32_t blk = min((t * kTile + quad * 16) >> c.block_log2, nb - 1);
+        ks_next = k_scale[blk];
+        vs_next = v_scale[blk];
+    };
+    auto ask_values = [&](uint32_t t) {
+        const uint32_t at = t * kTile + quad * 16, blk = min(at >> c.block_log2, nb - 1);
+        const uint8_t *src = values + (((uint64_t)blk * c.vdim + col) << c.block_log2) + (at & ((1u << c.block_log2) - 1));
+#pragma unroll
+        for (int v = 0; v < NV; v++)
+            if (v * 16 < (int)c.vdim) v_now[v] = *reinterpret_cast<const uint4 *>(src + ((uint64_t)(v * 16) << c.block_log2));
+    };
+    float4v total[RT][NV];
+    float maximum[RT], sum[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+        maximum[rt] = kNoMaximum;
+        sum[rt] = 0.0f;
+#pragma unroll
+        for (int v = 0; v < NV; v++) total[rt][v] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+#pragma unroll
+    for (int v = 0; v < NV; v++) v_now[v] = make_uint4(0, 0, 0, 0);
+    if (tile < end_tile) ask_keys(tile);
+    for (; tile < end_tile; tile += kStride) {
+#pragma unroll
+        for (int kt = 0; kt < 4; kt++)
+#pragma unroll
+            for (int l = 0; l < NL; l++) k_now[kt][l] = k_next[kt][l];
+        const float ks = ks_next, vs = vs_next;
+        ask_values(tile);
+        if (tile + kStride < end_tile) ask_keys(tile + kStride);
+        const int at0 = (int)(tile * kTile), mine = at0 + (int)quad * 16; // the tile's first position, the lane's
+        const bool masked = at0 < all_from || at0 + (int)kTile - 1 > all_to;
+        // scores^T
+        float4v score[RT][4];
+#pragma unroll
+        for (int kt = 0; kt < 4; kt++) {
+            half8v a[kSteps];
+#pragma unroll
+            for (int st = 0; st < kSteps; st++) a[st] = eight_of(k_now[kt][st / 2], st % 2);
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++) {
+                float4v s = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int piece = kPieces - 1; piece >= 0; piece--)
+#pragma unroll
+                    for (int st = 0; st < kSteps; st++) s = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[st], q[rt][piece][st], s, 0, 0, 0);
+                score[rt][kt] = s;
+            }
+        }
+        auto sees = [&](int rt, int i) { return mine + i >= begin[rt] && mine + i <= last[rt]; }; // i: of the lane's 16 positions
+        // the maxima
+        float factor[RT], largest[RT];
+        bool moves = false;
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
+            factor[rt] = row_factor[rt] * ks;
+            float m = -INFINITY;
+            if (masked) {
+#pragma unroll
+                for (int i = 0; i < 16; i++) m = sees(rt, i) ? fmaxf(m, score[rt][i / 4][i % 4]) : m;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; i++) m = fmaxf(m, score[rt][i / 4][i % 4]);
+            }
+            largest[rt] = m * factor[rt];
+            moves = moves || largest[rt] > maximum[rt] + 7.0f;
+        }
+        if (__any(moves)) {
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++) {
+                const float m = fmaxf(maximum[rt], quads_max(largest[rt])), down = __builtin_amdgcn_exp2f(maximum[rt] - m);
+                maximum[rt] = m;
+                sum[rt] *= down;
+#pragma unroll
+                for (int v = 0; v < NV; v++) total[rt][v] *= down;
+            }
+        }
+        // the weights
+        float weight[RT][16];
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
+            const float above = 8.0f - maximum[rt];
+#pragma unroll
+            for (int i = 0; i < 16; i++) weight[rt][i] = __builtin_amdgcn_exp2f(fmaf(score[rt][i / 4][i % 4], factor[rt], above));
+            if (masked) {
+#pragma unroll
+                for (int i = 0; i < 16; i++) weight[rt][i] = sees(rt, i) ? weight[rt][i] : 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < 16; i++) sum[rt] += weight[rt][i];
+        }
+        // NaN among the values of a tile that not every row sees whole
+        if (masked) {
+            uint32_t found = 0;
+#pragma unroll
+            for (int v = 0; v < NV; v++)
+#pragma unroll
+                for (int w = 0; w < 4; w++) found |= nan_bytes(word_of(v_now[v], w));
+            if (__any(found != 0)) {
+                half8v seen[RT][2];
+#pragma unroll
+                for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) seen[rt][i / 8][i % 8] = sees(rt, i) ? (_Float16)1.0f : (_Float16)0.0f;
+#pragma unroll
+                for (int v = 0; v < NV; v++) {
+                    uint32_t x[4], one[4]; // the codes without NaN; the code of 1 where one was
+#pragma unroll
+                    for (int w = 0; w < 4; w++) {
+                        const uint32_t bytes = (nan_bytes(word_of(v_now[v], w)) >> 7) * 255;
+                        x[w] = word_of(v_now[v], w) & ~bytes;
+                        one[w] = bytes & 0x38383838u;
+                    }
+                    v_now[v] = make_uint4(x[0], x[1], x[2], x[3]);
+#pragma unroll
+                    for (int rt = 0; rt < RT; rt++) {
+                        float4v n = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                        for (int st = 0; st < 2; st++) n = __builtin_amdgcn_mfma_f32_16x16x32_f16(eight_of(one[2 * st], one[2 * st + 1]), seen[rt][st], n, 0, 0, 0);
+#pragma unroll
+                        for (int i = 0; i < 4; i++) total[rt][v][i] = n[i] > 0.0f ? NAN : total[rt][v][i];
+                    }
+                }
+            }
+        }
+        // the value blocks' scales
+        int e = scale_exponent(vs), largest_e = e;
+        uint32_t passes = 1;
+        float block_factor = 1.0f;
+        if (c.block_log2 < 6) {
+            const int lowest = -1000;
+            const bool seen = mine + 15 >= any_from && mine <= any_to; // (a block that no row sees counts for nothing: its scale may be anything)
+            largest_e = quads_max(seen ? e : lowest);
+            const int smallest_e = -quads_max(seen ? -e : lowest);
+            e = seen ? e : largest_e;
+            if (largest_e == lowest) e = largest_e = 0;
+            else if (largest_e - smallest_e > 8) passes = 4;
+            block_factor = power_of_two(max(e - largest_e, -126));
+        }
+        for (uint32_t pass = 0; pass < passes; pass++) { // (the same for all lanes of a wave)
+            float out_factor = power_of_two(largest_e);
+            if (passes > 1) {
+                block_factor = quad == pass ? 1.0f : 0.0f;
+                out_factor = power_of_two(__shfl(e, (int)(pass * 16)));
+            }
+            half8v w[RT][kPieces][2];
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    float x = weight[rt][i];
+                    if (c.block_log2 < 6) x = passes > 1 && block_factor == 0.0f ? 0.0f : x * block_factor; // (NaN stays in its block)
+                    const _Float16 h = (_Float16)x;
+                    w[rt][0][i / 8][i % 8] = h;
+                    if (kPieces == 2) w[rt][kPieces - 1][i / 8][i % 8] = (_Float16)(x - (float)h);
+                }
+#pragma unroll
+            for (int v = 0; v < NV; v++) {
+                if (v * 16 >= (int)c.vdim) continue;
+                const half8v a[2] = {eight_of(v_now[v], 0), eight_of(v_now[v], 1)};
+#pragma unroll
+                for (int rt = 0; rt < RT; rt++) {
+                    float4v s = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int piece = kPieces - 1; piece >= 0; piece--)
+#pragma unroll
+                        for (int st = 0; st < 2; st++) s = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[st], w[rt][piece][st], s, 0, 0, 0);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) total[rt][v][i] = fmaf(s[i], out_factor, total[rt][v][i]);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) sum[rt] = quads_sum(sum[rt]);
+
+    // ---- the waves' results together: of two and two, then of the last two
+    if (!ROWS) {
+        __shared__ float4v shared_total[2][RT * NV][64];
+        __shared__ float2 shared_stats[2][RT][64];
+#pragma unroll
+        for (uint32_t half = 2; half >= 1; half /= 2) {
+            if (wave >= half && wave < 2 * half) {
+#pragma unroll
+                for (int rt = 0; rt < RT; rt++) {
+                    shared_stats[wave - half][rt][lane] = make_float2(maximum[rt], sum[rt]);
+#pragma unroll
+                    for (int v = 0; v < NV; v++) shared_total[wave - half][rt * NV + v][lane] = total[rt][v];
+                }
+            }
+            __syncthreads();
+            if (wave < half) {
+#pragma unroll
+                for (int rt = 0; rt < RT; rt++) {
+                    const float2 other = shared_stats[wave][rt][lane];
+                    const float m = fmaxf(maximum[rt], other.x), mine = __builtin_amdgcn_exp2f(maximum[rt] - m), its = __builtin_amdgcn_exp2f(other.x - m);
+                    maximum[rt] = m;
+                    sum[rt] = sum[rt] * mine + other.y * its;
+#pragma unroll
+                    for (int v = 0; v < NV; v++) total[rt][v] = total[rt][v] * mine + shared_total[wave][rt * NV + v][lane] * its;
+                }
+            }
+            __syncthreads();
+        }
+        if (wave > 0) return;
+    }
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+        const uint32_t r = row0 + rt * 16 + col;
+        if (r >= R) continue;
+        if (range.parts == 1) {
+            const float inv = sum[rt] == 0.0f ? 0.0f : 1.0f / sum[rt];
+            const uint32_t head = g * p.rep + r % p.rep;
+            T *const dst = static_cast<T *>(p.out) + row_token[rt] * p.out_pitch + head * c.vdim + quad * 4;
+            const bool whole = reinterpret_cast<uintptr_t>(p.out) % (4 * sizeof(T)) == 0 && p.out_pitch % 4 == 0;
+#pragma unroll
+            for (int v = 0; v < NV; v++) {
+                if (v * 16 >= (int)c.vdim) continue;
+                const float y[4] = {total[rt][v][0] * inv, total[rt][v][1] * inv, total[rt][v][2] * inv, total[rt][v][3] * inv};
+                store_elements<T, 4>(dst + v * 16, whole, y);
+            }
+        } else {
+            const uint64_t at = ((uint64_t)bg * p.splits + split) * p.rows + r;
+            if (quad == 0) p.stats[at] = make_float2(maximum[rt], sum[rt]);
+            float *const dst = p.parts + at * c.vdim + quad * 4;
+#pragma unroll
+            for (int v = 0; v < NV; v++)
+                if (v * 16 < (int)c.vdim) *reinterpret_cast<float4v *>(dst + v * 16) = total[rt][v];
+        }
+    }
+}
+
+template <class T> int launch_cache_attention_of(const LaunchOn &on, const CacheAttentionPlan &p) {
+    const dim3 grid(p.bgs * p.splits * p.row_blocks), block(64 * kWavesOfAttention);
+    const uint32_t nl = (std::max(p.cache.dim, p.cache.vdim) + 63) / 64;
+    auto launch = [&](auto kernel) { return on("cache attention launch", kernel, grid, block, p); };
+    if (nl == 1) return p.rows_by_wave ? launch(cache_attention_kernel<T, 1, 2, true>) : p.two_tiles ? launch(cache_attention_kernel<T, 1, 2, false>) : launch(cache_attention_kernel<T, 1, 1, false>);
+    if (nl == 2) return p.rows_by_wave ? launch(cache_attention_kernel<T, 2, 2, true>) : p.two_tiles ? launch(cache_attention_kernel<T, 2, 2, false>) : launch(cache_attention_kernel<T, 2, 1, false>);
+    return p.rows_by_wave ? launch(cache_attention_kernel<T, 4, 1, true>) : launch(cache_attention_kernel<T, 4, 1, false>);
+}
+template <class T> int load_cache_attention_of() {
+    hipFuncAttributes a;
+    CG_HIP(hipFuncGetAttributes(&a, reinterpret_cast<const void *>(cache_attention_kernel<T, 1, 1, false>)));
+    return CG_OK;
+}
+#endif
+
+int launch_cache_attention_f32(const LaunchOn &on, const CacheAttentionPlan &p);
+int launch_cache_attention_f16(const LaunchOn &on, const CacheAttentionPlan &p);
+int launch_cache_attention_bf16(const LaunchOn &on, const CacheAttentionPlan &p);
+int load_cache_attention_f32();
+int load_cache_attention_f16();
+int load_cache_attention_bf16();
+
+} // namespace cg

@@ -127,6 +127,13 @@ struct RotTable {
     Buffer *fine, *coarse;
     uint32_t coarse_n;
 };
+// cg_rotation_turns of a rotation, in memory; the oldest goes when there are kMostTurnTables.
+constexpr size_t kMostTurnTables = 16;
+struct TurnTable {
+    cg_rotation of;
+    Buffer *turns;
+    float magnitude;
+};
 } // namespace cg
 
 struct cg_backend {
@@ -168,6 +175,7 @@ struct cg_backend {
     cg::Buffer *iota = nullptr; // 0, 1, 2, ... : every arange is a view of it
     int64_t iota_len = 0;
     std::vector<cg::RotTable> rot_tables; // of the rotations that attention blocks have asked for
+    std::vector<cg::TurnTable> turn_tables; // ... that rotary blocks have
     bool fuse = true; // defer element-wise ops and fuse them (CG_FUSE=0 switches it off)
     bool aot = true;  // use the compiled kernels for listed programs (CG_AOT=0: interpreter only)
     uint64_t programs_compiled = 0, programs_interpreted = 0; // launches of fused programs, by kernel kind
@@ -595,6 +603,8 @@ enum ReduceKind : int { kSum = 0, kMax = 1, kArgmax = 2 };
 int launch_reduce(cg_backend *be, int kind, const cg_tensor *x, cg_tensor *out);
 // Asks for the device address of the fixed scratch array of cg_argmax_rows_noalloc on `device` (once per device).
 int noalloc_setup(int device);
+// Loads the kernels of the other entry points that allocate nothing on `device`, the calling thread's (block_cache.cpp).
+int cache_noalloc_setup(int device);
 int launch_topk(cg_backend *be, const cg_tensor *x, int64_t k, cg_tensor *vals, cg_tensor *idxs);
 // *flag_dev = any(x > 0) / any(x != y)
 int launch_any_positive(cg_backend *be, const cg_tensor *x);

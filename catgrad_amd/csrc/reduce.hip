@@ -610,8 +610,10 @@ int noalloc_setup(int device) {
     CG_HIP(hipSetDevice(device));
     long long *ptr = nullptr;
     const hipError_t e = hipGetSymbolAddress((void **)&ptr, HIP_SYMBOL(scratch));
+    const int rc = e == hipSuccess ? cache_noalloc_setup(device) : CG_OK;
     if (prev != device) (void)hipSetDevice(prev);
     if (e != hipSuccess) return hip_fail(e, "hipGetSymbolAddress(scratch)");
+    if (rc) return rc;
     if (!ptr) return fail(CG_ERR_DEVICE, "no device address for the scratch array on device %d", device);
     g_scratch_ptr[device].store(ptr, std::memory_order_release);
     return CG_OK;

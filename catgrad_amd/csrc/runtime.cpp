@@ -1244,6 +1244,8 @@ static void const_memo_clear(cg_backend *be) {
         buffer_release(t.coarse);
     }
     be->rot_tables.clear();
+    for (TurnTable &t : be->turn_tables) buffer_release(t.turns);
+    be->turn_tables.clear();
 }
 
 static void const_memo_insert(cg_backend *be, const std::string &key, Buffer *b) {
@@ -2377,6 +2379,7 @@ int cg_pool_stats(cg_backend *b, size_t *bytes_in_use, size_t *bytes_cached) {
     // what the backend keeps for itself (iota, rotations, results of constant programs) counts as cached
     size_t kept = b->const_bytes + (b->iota ? b->iota->cls : 0);
     for (const RotTable &t : b->rot_tables) kept += t.fine->cls + t.coarse->cls;
+    for (const TurnTable &t : b->turn_tables) kept += t.turns->cls;
     if (bytes_in_use) *bytes_in_use -= kept < *bytes_in_use ? kept : *bytes_in_use;
     if (bytes_cached) *bytes_cached += kept;
     return CG_OK;

@@ -251,6 +251,129 @@ int cg_concat(cg_backend *b, cg_tensor *x, cg_tensor *y, size_t dim, cg_tensor *
 /* `Backend::index` (mod.rs:94-99; ndarray.rs:466-487,571-579): gather along dim. */
 int cg_index(cg_backend *b, cg_tensor *x, size_t dim, cg_tensor *indices, cg_tensor **out);
 
+/* ---- a key / value cache in 8 bits (no counterpart in the reference) ------------------
+ * What a layer of a decoder does around attention when its cache is held as E4M3 codes (CG_F8's patterns): heads are turned by
+ * their tokens' positions, keys and values are appended, attention reads the codes.  For B sequences of S new tokens each.
+ *
+ *  k_codes [B, kv_heads, C, dim] and v_codes [B, kv_heads, C / block, vdim, block] hold room for C positions (values of `block`
+ *  neighbouring positions lie together for every channel: what a matrix instruction takes); k_scale and v_scale
+ *  [B, kv_heads, C / block] f32 a power of two 2^e for each block of positions and head: a code c stands for c * 2^e.
+ *  e is the smallest whole number from -117 to 119 with |x| <= 448 * 2^e for every finite value that the block's tokens had when
+ *  they were appended (448: the largest code); a value becomes the nearest code to x / 2^e (ties to even), infinities the largest,
+ *  NaN NaN.  Where new tokens make a block's e grow, the codes that it held are rounded to the new e.  A block whose first
+ *  position is appended starts anew, whatever its memory held.
+ *  (A power of two costs nothing: E4M3 values have the same relative precision at every scale, but for the smallest, and a scaled
+ *  code is exact in 32 bits, so a cache's contents do not depend on how its tokens were portioned except where e grew.)
+ *
+ *  dim and vdim are multiples of 16 up to 256, block is 16, 32, 64 or 128, C a multiple of it. */
+
+/* How positions turn heads: of the first `dims` (even) values of a head the pairs (2 i, 2 i + 1) with `interleaved`, else
+ * (i, i + dims / 2), are turned by position * f_i and multiplied by the magnitude; f_i = base^(-2 i / dims) is scaled for contexts
+ * longer than `original` positions:
+ *  CG_ROTATION_LINEAR: f_i / factor;
+ *  CG_ROTATION_BANDS (rope.rs:231-310): f_i (p + (1 - p) / factor), p = (original * f_i / 2 pi - low) / (high - low) within 0 .. 1;
+ *  CG_ROTATION_RAMP: f_i ((1 - p) + p / factor), p = (i - a) / (b - a) within 0 .. 1, a and b the pairs that turn `high` and `low`
+ *  times within `original` positions, rounded down and up; its magnitude is 0.1 ln(factor) + 1, the others' 1, where `magnitude` is 0. */
+typedef enum cg_rotation_scaling { CG_ROTATION_PLAIN = 0, CG_ROTATION_LINEAR = 1, CG_ROTATION_BANDS = 2, CG_ROTATION_RAMP = 3 } cg_rotation_scaling;
+typedef struct cg_rotation {
+    size_t dims;
+    int interleaved;
+    cg_rotation_scaling scaling;
+    double base, factor, low, high, original, magnitude;
+} cg_rotation;
+/* f_i / 2 pi (turns a position) for i < dims / 2, and the magnitude.  Host memory; needs no device. */
+int cg_rotation_turns(const cg_rotation *r, double *turns, float *magnitude);
+
+/* q [B, S, heads * dim] and k [B, S, kv_heads * dim] (k: may be null, then k_out is left alone) at the positions position ..
+ * position + S - 1. */
+typedef struct cg_rotary_args {
+    cg_tensor *q, *k;
+    size_t heads, kv_heads, dim, position;
+    cg_rotation rotation;
+} cg_rotary_args;
+int cg_block_rotary(cg_backend *b, const cg_rotary_args *a, cg_tensor **q_out, cg_tensor **k_out);
+
+/* k [B, S, kv_heads * dim], v [B, S, kv_heads * vdim] at the positions position .. position + S - 1 <= C - 1.  The caches are
+ * written in place where the caller's are the only references to them (cg_zeros makes an empty one), else copied. */
+typedef struct cg_cache_append_args {
+    cg_tensor *k, *v, *k_codes, *v_codes, *k_scale, *v_scale;
+    size_t position;
+} cg_cache_append_args;
+int cg_block_cache_append(cg_backend *b, const cg_cache_append_args *a, cg_tensor **k_codes_out, cg_tensor **v_codes_out, cg_tensor **k_scale_out,
+                          cg_tensor **v_scale_out);
+
+/* out [B, S, heads * vdim] = softmax(scale * q . k) v, q [B, S, heads * dim] at the positions position .. position + S - 1, which
+ * the cache holds already: a query sees the positions up to its own, of which a window leaves the last `window` (0: all).
+ * Consecutive heads / kv_heads query heads share a key / value head. */
+typedef struct cg_cache_attention_args {
+    cg_tensor *q, *k_codes, *v_codes, *k_scale, *v_scale;
+    size_t heads, position, window;
+    float scale;
+} cg_cache_attention_args;
+int cg_block_cache_attention(cg_backend *b, const cg_cache_attention_args *a, cg_tensor **out);
+
+/* The same for callers that cannot allocate device memory (see cg_argmax_rows_noalloc): all arrays lie in the caller's device
+ * memory, kernels are queued on `stream` (a hipStream_t; null = the default stream) of `device`, and the calls allocate nothing,
+ * free nothing and do not wait.  cg_noalloc_setup(device), or cg_backend_create on it, has returned CG_OK before.  Calls share no
+ * memory but what they are given: they may overlap in time where that is apart, workspaces included.
+ *
+ * Batches may be ragged: sequence b holds held[b] positions (held null: `position` for all) and brings counts[b] <= tokens new
+ * ones (counts null: `tokens`; more count as `tokens`), which stand at the positions held[b] .. held[b] + counts[b] - 1.  Rows of q, k, v and results are
+ * [sequences, tokens]; those behind counts[b] are not read, and results there are left as they were.  q, k, v and results are of one
+ * dtype, CG_F32, CG_F16 or CG_BF16 (2-byte elements); pitches are the distance from token to token in elements (0: dense). */
+typedef struct cg_token_batch {
+    size_t sequences, tokens, position;
+    const uint32_t *held, *counts;
+} cg_token_batch;
+typedef struct cg_cache8 { /* codes at multiples of 16 bytes */
+    uint8_t *k_codes, *v_codes;
+    float *k_scale, *v_scale;
+    size_t kv_heads, dim, vdim, capacity, block;
+} cg_cache8;
+
+/* turns: device memory, from cg_rotation_turns or of a rule of the caller's own.  k may be null.  Results may be q and k
+ * themselves, with their pitches. */
+typedef struct cg_rotary_rows {
+    cg_token_batch batch;
+    cg_dtype dtype;
+    const void *q, *k;
+    void *q_out, *k_out;
+    size_t q_pitch, k_pitch, q_out_pitch, k_out_pitch;
+    size_t heads, kv_heads, dim, rot_dims;
+    int interleaved;
+    float magnitude;
+    const double *turns;
+} cg_rotary_rows;
+int cg_rotary_noalloc(int device, const cg_rotary_rows *a, void *stream);
+
+/* Tokens whose position is `capacity` or more are not stored. */
+typedef struct cg_cache_append_rows {
+    cg_token_batch batch;
+    cg_dtype dtype;
+    const void *k, *v;
+    size_t k_pitch, v_pitch;
+    cg_cache8 cache;
+} cg_cache_append_rows;
+int cg_cache_append_noalloc(int device, const cg_cache_append_rows *a, void *stream);
+
+/* batch: as it was for the append of the same tokens.  A query that sees nothing (its window lies behind the capacity) gives
+ * zeros.  workspace: device memory of at least the bytes that cg_cache_attention_workspace says for the same sizes, at a multiple of
+ * 16 bytes; its contents do not matter before or after the call.  (0 bytes: it may be null.) */
+typedef struct cg_cache_attention_rows {
+    cg_token_batch batch;
+    cg_dtype dtype;
+    const void *q;
+    void *out;
+    size_t q_pitch, out_pitch, heads;
+    cg_cache8 cache;
+    float scale;
+    size_t window;
+    void *workspace;
+    size_t workspace_bytes;
+} cg_cache_attention_rows;
+int cg_cache_attention_workspace(const cg_cache_attention_rows *a, size_t *bytes);
+int cg_cache_attention_noalloc(int device, const cg_cache_attention_rows *a, void *stream);
+
 /* ---- decoder blocks (no counterpart in the reference) ---------------------------
  * Steps of a decoder layer that the trait's ops cannot express without writing every intermediate out, or not at all
  * without an op per token (a recurrence).  Each is one call with its mechanisms as parameters; an absent mechanism is a

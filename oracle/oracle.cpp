@@ -1828,3 +1828,340 @@ int cg_block_channel_delta(cg_backend *, const cg_channel_delta_args *a, cg_tens
 }
 
 } // extern "C"
+
+// ---- rotary positions and the 8-bit key / value cache (their section of include/catgrad_hip.h): plain loops in double ----
+// The arrays of the entry points that allocate nothing lie in host memory here.
+namespace {
+
+double element(cg_dtype dt, const void *p, size_t i) {
+    if (dt == CG_F32) return static_cast<const float *>(p)[i];
+    const uint16_t h = static_cast<const uint16_t *>(p)[i];
+    return float_of(dt == CG_BF16 ? (uint32_t)h << 16 : f16_bits_to_f32(h));
+}
+void put(cg_dtype dt, void *p, size_t i, double v) {
+    const uint32_t u = bits_of((float)v);
+    if (dt == CG_F32) static_cast<float *>(p)[i] = (float)v;
+    else static_cast<uint16_t *>(p)[i] = dt == CG_BF16 ? f32_to_bf16_bits(u) : f32_to_f16_bits(u);
+}
+double code_value(uint8_t c) { return float_of(f8e4m3_bits_to_f32(c)); }
+// the nearest code, ties to even, within its range (the values here are codes, or 32-bit floats, times a power of two: exact as floats
+// where the result is not zero)
+uint8_t nearest_code(double v) { return f32_to_f8e4m3_bits(bits_of((float)v)); }
+
+size_t held_by(const cg_token_batch &t, size_t b) { return t.held ? t.held[b] : t.position; }
+size_t count_of(const cg_token_batch &t, size_t b) { return t.counts ? std::min<size_t>(t.counts[b], t.tokens) : t.tokens; }
+bool some(const cg_token_batch &t) { return t.sequences != 0 && t.tokens != 0; }
+bool element_type(cg_dtype dt) { return dt == CG_F32 || dt == CG_F16 || dt == CG_BF16; }
+
+int turn_heads(const cg_token_batch &t, cg_dtype dt, const void *x, void *y, size_t x_pitch, size_t y_pitch, size_t heads, const cg_rotary_rows &a) {
+    const size_t half = a.rot_dims / 2;
+    for (size_t b = 0; b < t.sequences; b++)
+        for (size_t s = 0; s < count_of(t, b); s++)
+            for (size_t h = 0; h < heads; h++) {
+                const size_t from = (b * t.tokens + s) * x_pitch + h * a.dim, to = (b * t.tokens + s) * y_pitch + h * a.dim;
+                for (size_t i = 0; i < half; i++) {
+                    const size_t u = a.interleaved ? 2 * i : i, w = a.interleaved ? 2 * i + 1 : half + i;
+                    const double turns = (double)(held_by(t, b) + s) * a.turns[i], angle = 6.283185307179586476925 * (turns - std::rint(turns));
+                    const double c = std::cos(angle) * a.magnitude, d = std::sin(angle) * a.magnitude, p = element(dt, x, from + u), q = element(dt, x, from + w);
+                    put(dt, y, to + u, p * c - q * d);
+                    put(dt, y, to + w, q * c + p * d);
+                }
+                for (size_t i = a.rot_dims; i < a.dim; i++) put(dt, y, to + i, element(dt, x, from + i));
+            }
+    return CG_OK;
+}
+int bad_rotation(size_t heads, size_t kv_heads, size_t dim, size_t rot) {
+    if (heads < 1 || heads > 4096 || kv_heads > 4096 || dim < 2 || dim > 4096 || rot < 2 || rot % 2 || rot > dim || rot > 512) return fail(CG_ERR_ARG, "rotary: bad sizes");
+    return CG_OK;
+}
+int bad_cache(const cg_cache8 &c) {
+    for (size_t n : {c.dim, c.vdim})
+        if (n < 16 || n > 256 || n % 16) return fail(CG_ERR_UNSUPPORTED, "cache: heads of 16, 32, .. 256 channels");
+    if (c.block != 16 && c.block != 32 && c.block != 64 && c.block != 128) return fail(CG_ERR_UNSUPPORTED, "cache: blocks of 16, 32, 64 or 128 positions");
+    if (c.capacity < c.block || c.capacity % c.block) return fail(CG_ERR_SHAPE, "cache: whole blocks");
+    if (c.kv_heads < 1 || c.kv_heads > 4096) return fail(CG_ERR_ARG, "cache: bad head counts");
+    return CG_OK;
+}
+int pitch_or(size_t pitch, size_t width, size_t *out) {
+    if (pitch && pitch < width) return fail(CG_ERR_ARG, "rows lie closer than they are wide");
+    *out = pitch ? pitch : width;
+    return CG_OK;
+}
+
+// Where the code of (head bg, position, channel) lies.
+size_t code_at(const cg_cache8 &c, bool values, size_t bg, size_t pos, size_t d) {
+    if (!values) return (bg * c.capacity + pos) * c.dim + d;
+    return ((bg * (c.capacity / c.block) + pos / c.block) * c.vdim + d) * c.block + pos % c.block;
+}
+void append_rows(const cg_token_batch &t, cg_dtype dt, const void *x, size_t pitch, const cg_cache8 &c, bool values) {
+    const size_t W = values ? c.vdim : c.dim, nb = c.capacity / c.block;
+    uint8_t *codes = values ? c.v_codes : c.k_codes;
+    float *scales = values ? c.v_scale : c.k_scale;
+    for (size_t b = 0; b < t.sequences; b++)
+        for (size_t g = 0; g < c.kv_heads; g++) {
+            const size_t held = held_by(t, b), end = std::min(held + count_of(t, b), c.capacity), bg = b * c.kv_heads + g;
+            for (size_t j = held / c.block; j * c.block < end && j < nb; j++) {
+                const size_t p0 = std::max(held, j * c.block), p1 = std::min(end, (j + 1) * c.block);
+                if (p0 >= p1) continue;
+                auto fresh = [&](size_t pos, size_t d) { return element(dt, x, (b * t.tokens + pos - held) * pitch + g * W + d); };
+                double size = 0.0;
+                for (size_t p = p0; p < p1; p++)
+                    for (size_t d = 0; d < W; d++)
+                        if (std::isfinite(fresh(p, d))) size = std::max(size, std::fabs(fresh(p, d)));
+                int e = -117;
+                while (e < 119 && size > std::ldexp(448.0, e)) e++;
+                int had = -117;
+                if (p0 > j * c.block) {
+                    had = std::min(119, std::max(-117, (int)(bits_of(scales[bg * nb + j]) >> 23 & 255) - 127));
+                    e = std::max(e, had);
+                    for (size_t p = j * c.block; p < p0 && e > had; p++)
+                        for (size_t d = 0; d < W; d++) {
+                            uint8_t &k = codes[code_at(c, values, bg, p, d)];
+                            k = nearest_code(std::ldexp(code_value(k), had - e));
+                        }
+                }
+                for (size_t p = p0; p < p1; p++)
+                    for (size_t d = 0; d < W; d++) codes[code_at(c, values, bg, p, d)] = nearest_code(std::ldexp(fresh(p, d), -e));
+                scales[bg * nb + j] = std::ldexp(1.0f, e);
+            }
+        }
+}
+
+void attend_rows(const cg_cache_attention_rows &a, size_t q_pitch, size_t out_pitch) {
+    const cg_cache8 &c = a.cache;
+    const size_t rep = a.heads / c.kv_heads, nb = c.capacity / c.block;
+    for (size_t b = 0; b < a.batch.sequences; b++)
+        for (size_t s = 0; s < count_of(a.batch, b); s++)
+            for (size_t h = 0; h < a.heads; h++) {
+                const size_t bg = b * c.kv_heads + h / rep, at = held_by(a.batch, b) + s, end = std::min(at + 1, c.capacity);
+                const size_t lo = std::min(end, a.window && at + 1 > a.window ? at + 1 - a.window : 0), row = b * a.batch.tokens + s;
+                std::vector<double> w(end - lo), o(c.vdim, 0.0);
+                double m = -std::numeric_limits<double>::infinity(), sum = 0.0;
+                for (size_t j = lo; j < end; j++) {
+                    double x = 0.0;
+                    for (size_t d = 0; d < c.dim; d++) x += element(a.dtype, a.q, row * q_pitch + h * c.dim + d) * code_value(c.k_codes[code_at(c, false, bg, j, d)]);
+                    w[j - lo] = x * a.scale * c.k_scale[bg * nb + j / c.block];
+                    m = w[j - lo] > m || w[j - lo] != w[j - lo] ? w[j - lo] : m;
+                }
+                for (double &x : w) sum += x = std::exp(x - m);
+                for (size_t j = lo; j < end; j++)
+                    for (size_t d = 0; d < c.vdim; d++) o[d] += w[j - lo] / sum * code_value(c.v_codes[code_at(c, true, bg, j, d)]) * c.v_scale[bg * nb + j / c.block];
+                for (size_t d = 0; d < c.vdim; d++) put(a.dtype, a.out, row * out_pitch + h * c.vdim + d, o[d]);
+            }
+}
+
+// A cache's tensors as the arrays above, and back.
+struct CacheArrays {
+    std::vector<uint8_t> k, v;
+    Vec<float> ks, vs;
+    cg_cache8 c{};
+    int take(size_t B, const cg_tensor *kc, const cg_tensor *vc, const cg_tensor *kt, const cg_tensor *vt) {
+        if (kc->dt != CG_F8 || vc->dt != CG_F8 || kt->dt != CG_F32 || vt->dt != CG_F32) return fail(CG_ERR_DTYPE, "cache: codes are f8, scales f32");
+        if (kc->rank != 4 || vc->rank != 5 || kt->rank != 3 || vt->rank != 3) return fail(CG_ERR_SHAPE, "cache: bad ranks");
+        c.kv_heads = kc->dims[1];
+        c.capacity = kc->dims[2];
+        c.dim = kc->dims[3];
+        c.vdim = vc->dims[3];
+        c.block = vc->dims[4];
+        if (kc->dims[0] != B || vc->dims[0] != B || vc->dims[1] != c.kv_heads || vc->dims[2] * c.block != c.capacity || c.block < 1) return fail(CG_ERR_SHAPE, "cache: incompatible caches");
+        for (const cg_tensor *s : {kt, vt})
+            if (s->dims[0] != B || s->dims[1] != c.kv_heads || s->dims[2] != vc->dims[2]) return fail(CG_ERR_SHAPE, "cache: incompatible scales");
+        if (int rc = bad_cache(c)) return rc;
+        auto bytes = [](const cg_tensor *t) {
+            Vec<uint32_t> w = dense<uint32_t>(t);
+            std::vector<uint8_t> r(w.size());
+            for (size_t i = 0; i < w.size(); i++) r[i] = f32_to_f8e4m3_bits(w[i]);
+            return r;
+        };
+        k = bytes(kc);
+        v = bytes(vc);
+        ks = dense<float>(kt);
+        vs = dense<float>(vt);
+        c.k_codes = k.data();
+        c.v_codes = v.data();
+        c.k_scale = ks.data();
+        c.v_scale = vs.data();
+        return CG_OK;
+    }
+};
+
+} // namespace
+
+extern "C" {
+
+int cg_rotation_turns(const cg_rotation *r, double *turns, float *magnitude) {
+    if (!r || !turns || !magnitude) return fail(CG_ERR_ARG, "null argument");
+    if (r->dims < 2 || r->dims % 2 || r->dims > 512 || !(r->base > 0.0) || !std::isfinite(r->base) || !(r->magnitude >= 0.0)) return fail(CG_ERR_ARG, "rotation: bad sizes");
+    if ((int)r->scaling < CG_ROTATION_PLAIN || r->scaling > CG_ROTATION_RAMP) return fail(CG_ERR_ARG, "rotation: unknown scaling");
+    if (r->scaling != CG_ROTATION_PLAIN && !(r->factor > 0.0)) return fail(CG_ERR_ARG, "rotation: bad factor");
+    if (r->scaling >= CG_ROTATION_BANDS && (!(r->original > 0.0) || !(r->low > 0.0) || !(r->high > r->low))) return fail(CG_ERR_ARG, "rotation: bad limits");
+    if (r->scaling == CG_ROTATION_RAMP && r->base <= 1.0) return fail(CG_ERR_ARG, "rotation: bad base");
+    const double pi2 = 6.283185307179586476925;
+    for (size_t i = 0; i < r->dims / 2; i++) {
+        const double f = std::exp(-2.0 * (double)i / (double)r->dims * std::log(r->base));
+        double g = f;
+        if (r->scaling == CG_ROTATION_LINEAR) g = f / r->factor;
+        if (r->scaling == CG_ROTATION_BANDS) { // rope.rs:231-310
+            const double wave = pi2 / f, p = (r->original / wave - r->low) / (r->high - r->low);
+            g = wave < r->original / r->high ? f : wave > r->original / r->low ? f / r->factor : (1.0 - p) * f / r->factor + p * f;
+        }
+        if (r->scaling == CG_ROTATION_RAMP) {
+            auto pair = [&](double times) { return (double)r->dims / 2.0 * std::log(r->original / (pi2 * times)) / std::log(r->base); };
+            const double lo = std::max(0.0, std::floor(pair(r->high))), hi = std::max(lo + 1e-3, std::min((double)r->dims - 1.0, std::ceil(pair(r->low))));
+            const double p = std::min(1.0, std::max(0.0, ((double)i - lo) / (hi - lo)));
+            g = f / r->factor * p + f * (1.0 - p);
+        }
+        turns[i] = g / pi2;
+    }
+    *magnitude = (float)(r->magnitude > 0.0 ? r->magnitude : r->scaling == CG_ROTATION_RAMP ? 0.1 * std::log(r->factor) + 1.0 : 1.0);
+    return CG_OK;
+}
+
+int cg_rotary_noalloc(int, const cg_rotary_rows *a, void *) {
+    if (!a) return fail(CG_ERR_ARG, "null argument");
+    if (!element_type(a->dtype)) return fail(CG_ERR_DTYPE, "rotary: elements are f32, f16 or bf16");
+    if (int rc = bad_rotation(a->heads, a->k ? a->kv_heads : 0, a->dim, a->rot_dims)) return rc;
+    if (a->k && a->kv_heads < 1) return fail(CG_ERR_ARG, "rotary: bad sizes");
+    if (!some(a->batch)) return CG_OK;
+    if (!a->q || !a->q_out || (a->k && !a->k_out) || !a->turns) return fail(CG_ERR_ARG, "null argument");
+    size_t qp = 0, qo = 0, kp = 0, ko = 0;
+    if (int rc = pitch_or(a->q_pitch, a->heads * a->dim, &qp)) return rc;
+    if (int rc = pitch_or(a->q_out_pitch, a->heads * a->dim, &qo)) return rc;
+    if (int rc = turn_heads(a->batch, a->dtype, a->q, a->q_out, qp, qo, a->heads, *a)) return rc;
+    if (!a->k) return CG_OK;
+    if (int rc = pitch_or(a->k_pitch, a->kv_heads * a->dim, &kp)) return rc;
+    if (int rc = pitch_or(a->k_out_pitch, a->kv_heads * a->dim, &ko)) return rc;
+    return turn_heads(a->batch, a->dtype, a->k, a->k_out, kp, ko, a->kv_heads, *a);
+}
+
+int cg_cache_append_noalloc(int, const cg_cache_append_rows *a, void *) {
+    if (!a) return fail(CG_ERR_ARG, "null argument");
+    if (!element_type(a->dtype)) return fail(CG_ERR_DTYPE, "cache append: elements are f32, f16 or bf16");
+    if (!some(a->batch)) return CG_OK;
+    if (int rc = bad_cache(a->cache)) return rc;
+    const cg_cache8 &c = a->cache;
+    if (!a->k || !a->v || !c.k_codes || !c.v_codes || !c.k_scale || !c.v_scale) return fail(CG_ERR_ARG, "null argument");
+    size_t kp = 0, vp = 0;
+    if (int rc = pitch_or(a->k_pitch, c.kv_heads * c.dim, &kp)) return rc;
+    if (int rc = pitch_or(a->v_pitch, c.kv_heads * c.vdim, &vp)) return rc;
+    append_rows(a->batch, a->dtype, a->k, kp, c, false);
+    append_rows(a->batch, a->dtype, a->v, vp, c, true);
+    return CG_OK;
+}
+
+int cg_cache_attention_workspace(const cg_cache_attention_rows *a, size_t *bytes) {
+    if (!a || !bytes) return fail(CG_ERR_ARG, "null argument");
+    *bytes = 0;
+    if (!some(a->batch)) return CG_OK;
+    return bad_cache(a->cache);
+}
+
+int cg_cache_attention_noalloc(int, const cg_cache_attention_rows *a, void *) {
+    if (!a) return fail(CG_ERR_ARG, "null argument");
+    if (!some(a->batch)) return CG_OK;
+    if (!element_type(a->dtype)) return fail(CG_ERR_DTYPE, "cache attention: elements are f32, f16 or bf16");
+    if (int rc = bad_cache(a->cache)) return rc;
+    const cg_cache8 &c = a->cache;
+    if (a->heads < 1 || a->heads > 4096 || a->heads % c.kv_heads || !std::isfinite(a->scale)) return fail(CG_ERR_ARG, "cache attention: bad head counts or scale");
+    if (!a->q || !a->out || !c.k_codes || !c.v_codes || !c.k_scale || !c.v_scale) return fail(CG_ERR_ARG, "null argument");
+    size_t qp = 0, op = 0;
+    if (int rc = pitch_or(a->q_pitch, a->heads * c.dim, &qp)) return rc;
+    if (int rc = pitch_or(a->out_pitch, a->heads * c.vdim, &op)) return rc;
+    attend_rows(*a, qp, op);
+    return CG_OK;
+}
+
+int cg_block_rotary(cg_backend *, const cg_rotary_args *a, cg_tensor **q_out, cg_tensor **k_out) {
+    if (!a) return fail(CG_ERR_ARG, "null argument");
+    Owned own{{a->q, a->k}};
+    if (!a->q || !q_out || (a->k && !k_out)) return fail(CG_ERR_ARG, "null argument");
+    if (int rc = bad_rotation(a->heads, a->k ? a->kv_heads : 0, a->dim, a->rotation.dims)) return rc;
+    if (a->q->rank != 3 || (a->k && (a->k->rank != 3 || a->kv_heads < 1))) return fail(CG_ERR_SHAPE, "block_rotary: bad ranks");
+    const size_t B = a->q->dims[0], S = a->q->dims[1];
+    if (a->q->dims[2] != a->heads * a->dim || !B || !S || (a->k && (a->k->dims[0] != B || a->k->dims[1] != S || a->k->dims[2] != a->kv_heads * a->dim)))
+        return fail(CG_ERR_SHAPE, "block_rotary: incompatible shapes");
+    double turns[256];
+    cg_rotary_rows r{};
+    if (int rc = cg_rotation_turns(&a->rotation, turns, &r.magnitude)) return rc;
+    r.batch = {B, S, a->position, nullptr, nullptr};
+    r.dim = a->dim;
+    r.rot_dims = a->rotation.dims;
+    r.interleaved = a->rotation.interleaved;
+    r.turns = turns;
+    auto turned = [&](const cg_tensor *t, size_t heads) {
+        Vec<float> x = dense<float>(t);
+        cg_tensor *o = new_tensor(CG_F32, t->dims, 3);
+        turn_heads(r.batch, CG_F32, x.data(), data_of<float>(o), heads * a->dim, heads * a->dim, heads, r);
+        return o;
+    };
+    *q_out = turned(a->q, a->heads);
+    if (a->k) *k_out = turned(a->k, a->kv_heads);
+    return CG_OK;
+}
+
+int cg_block_cache_append(cg_backend *, const cg_cache_append_args *a, cg_tensor **k_codes_out, cg_tensor **v_codes_out, cg_tensor **k_scale_out,
+                          cg_tensor **v_scale_out) {
+    if (!a) return fail(CG_ERR_ARG, "null argument");
+    Owned own{{a->k, a->v, a->k_codes, a->v_codes, a->k_scale, a->v_scale}};
+    for (const cg_tensor *t : own.t)
+        if (!t) return fail(CG_ERR_ARG, "null argument");
+    if (!k_codes_out || !v_codes_out || !k_scale_out || !v_scale_out) return fail(CG_ERR_ARG, "null argument");
+    if (a->k->rank != 3 || a->v->rank != 3) return fail(CG_ERR_SHAPE, "block_cache_append: bad ranks");
+    const size_t B = a->k->dims[0], S = a->k->dims[1];
+    CacheArrays m;
+    if (int rc = m.take(B, a->k_codes, a->v_codes, a->k_scale, a->v_scale)) return rc;
+    if (!B || !S || a->v->dims[0] != B || a->v->dims[1] != S || a->k->dims[2] != m.c.kv_heads * m.c.dim || a->v->dims[2] != m.c.kv_heads * m.c.vdim)
+        return fail(CG_ERR_SHAPE, "block_cache_append: incompatible shapes");
+    if (a->position > m.c.capacity || a->position + S > m.c.capacity) return fail(CG_ERR_RANGE, "block_cache_append: the cache has no room for the positions");
+    const cg_token_batch t = {B, S, a->position, nullptr, nullptr};
+    Vec<float> k = dense<float>(a->k), v = dense<float>(a->v);
+    append_rows(t, CG_F32, k.data(), a->k->dims[2], m.c, false);
+    append_rows(t, CG_F32, v.data(), a->v->dims[2], m.c, true);
+    auto codes = [](const std::vector<uint8_t> &x, const cg_tensor *like) {
+        cg_tensor *o = new_tensor(CG_F8, like->dims, like->rank);
+        for (size_t i = 0; i < x.size(); i++) o->st->data[i] = f8e4m3_bits_to_f32(x[i]);
+        return o;
+    };
+    auto scales = [](const Vec<float> &x, const cg_tensor *like) {
+        cg_tensor *o = new_tensor(CG_F32, like->dims, like->rank);
+        std::copy(x.begin(), x.end(), data_of<float>(o));
+        return o;
+    };
+    *k_codes_out = codes(m.k, a->k_codes);
+    *v_codes_out = codes(m.v, a->v_codes);
+    *k_scale_out = scales(m.ks, a->k_scale);
+    *v_scale_out = scales(m.vs, a->v_scale);
+    return CG_OK;
+}
+
+int cg_block_cache_attention(cg_backend *, const cg_cache_attention_args *a, cg_tensor **out) {
+    if (!a) return fail(CG_ERR_ARG, "null argument");
+    Owned own{{a->q, a->k_codes, a->v_codes, a->k_scale, a->v_scale}};
+    for (const cg_tensor *t : own.t)
+        if (!t) return fail(CG_ERR_ARG, "null argument");
+    if (!out) return fail(CG_ERR_ARG, "null argument");
+    if (a->q->rank != 3) return fail(CG_ERR_SHAPE, "block_cache_attention: bad ranks");
+    const size_t B = a->q->dims[0], S = a->q->dims[1];
+    CacheArrays m;
+    if (int rc = m.take(B, a->k_codes, a->v_codes, a->k_scale, a->v_scale)) return rc;
+    if (a->heads < 1 || a->heads > 4096 || a->heads % m.c.kv_heads || !std::isfinite(a->scale)) return fail(CG_ERR_ARG, "block_cache_attention: bad head counts or scale");
+    if (!B || !S || a->q->dims[2] != a->heads * m.c.dim) return fail(CG_ERR_SHAPE, "block_cache_attention: incompatible shapes");
+    if (a->position > m.c.capacity || a->position + S > m.c.capacity) return fail(CG_ERR_RANGE, "block_cache_attention: the cache does not hold the positions");
+    Vec<float> q = dense<float>(a->q);
+    const size_t od[3] = {B, S, a->heads * m.c.vdim};
+    cg_tensor *o = new_tensor(CG_F32, od, 3);
+    cg_cache_attention_rows r{};
+    r.batch = {B, S, a->position, nullptr, nullptr};
+    r.dtype = CG_F32;
+    r.q = q.data();
+    r.out = data_of<float>(o);
+    r.heads = a->heads;
+    r.cache = m.c;
+    r.scale = a->scale;
+    r.window = a->window;
+    attend_rows(r, a->q->dims[2], od[2]);
+    *out = o;
+    return CG_OK;
+}
+
+} // extern "C"
