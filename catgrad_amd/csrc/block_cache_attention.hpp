@@ -15,11 +15,12 @@
 // in [2^7, 2^8), and is one 16-bit float a value, or with 32-bit inputs the sum of two (2^-23 of the row's largest; 16-bit inputs are
 // exact but where they lie 2^22 below it).  A block's scale multiplies the scores in 32 bits.  Weights are exp2(score - m + 8) <= 2^15
 // with m the running maximum, which moves only where a score is 7 or more above it (most tiles move none: then nothing is
-// rescaled), as one 16-bit float (2^-12) or two (2^-23).  The second product of a tile starts from zero and is added to the
-// total by a vector instruction, with the value block's scale: the matrix instruction cuts its sums off, which over a long
-// cache would move all of them to one side, and the total is never in units of an earlier block's scale.  In blocks of 16 or 32 positions a tile's
-// scales differ: weights are multiplied by 2^(e - the largest e), and where those are more than 2^8 apart every block is a product of
-// its own.  The sum of weights is taken in 32 bits, of the weights before they are rounded.
+// rescaled), as one 16-bit float (2^-12) or two (2^-23), and so is their sum, by the same instruction from ones.
+// Totals are in units of a value block's scale, the codes' own scales being applied as they are widened: exact up to 2^-15 of the
+// unit.  A tile whose scale is larger, or smaller than that, has the totals rescaled to its own (most tiles have none); one whose blocks
+// of 16 or 32 positions lie farther apart is taken a block at a time.  With 16-bit results the instruction adds to the totals
+// itself.  It cuts its sums off, a thousand times for 32000 positions: 2^-15, which such results do not see; with 32-bit results the product of
+// a tile starts from zero and is added by a vector instruction.
 //
 // Positions that a row does not see: their weights are set to zero, and since zero times NaN is NaN, a tile that not all rows
 // see whole has its NaN codes of values taken out, and put back into the totals of the rows that do see them.
@@ -37,6 +38,8 @@ typedef float float4v __attribute__((ext_vector_type(4)));
 constexpr uint32_t kTile = 64;           // positions of a wave's tile
 constexpr uint32_t kWavesOfAttention = 4;
 constexpr float kNoMaximum = -3.0e38f;   // of a row that has seen nothing
+// A code times 2^-15 is exact as a 16-bit float (whole multiples of 2^-9, 2^-24); totals of 2^41 units times 2^80 are finite.
+constexpr int kExact = 15, kMostDown = 80;
 // The fewest tiles worth a part of their own, with the waves sharing a row's tiles and without.
 constexpr uint32_t kLeastTilesShared = 8, kLeastTilesRows = 8;
 
@@ -57,16 +60,19 @@ __device__ __forceinline__ KeyRange key_range(const CacheAttentionPlan &p, uint6
 }
 
 #ifdef __HIPCC__
-// codes 2 i, 2 i + 1 of a word as 16-bit floats (exact)
-template <bool HIGH> __device__ __forceinline__ half2v two_of(uint32_t codes) { return __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)codes, 1.0f, HIGH); }
-__device__ __forceinline__ half8v eight_of(uint32_t lo, uint32_t hi) {
-    const half2v a = two_of<false>(lo), b = two_of<true>(lo), c = two_of<false>(hi), d = two_of<true>(hi);
+// codes 2 i, 2 i + 1 of a word, times a power of two, as 16-bit floats (exact with 1)
+template <bool HIGH> __device__ __forceinline__ half2v two_of(uint32_t codes, float scale) { return __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)codes, scale, HIGH); }
+__device__ __forceinline__ half8v eight_of(uint32_t lo, uint32_t hi, float scale) {
+    const half2v a = two_of<false>(lo, scale), b = two_of<true>(lo, scale), c = two_of<false>(hi, scale), d = two_of<true>(hi, scale);
     return half8v{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 __device__ __forceinline__ uint32_t word_of(const uint4 &v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 // the k-th eight codes of sixteen
-__device__ __forceinline__ half8v eight_of(const uint4 &v, int k) { return eight_of(word_of(v, 2 * k), word_of(v, 2 * k + 1)); }
+__device__ __forceinline__ half8v eight_of(const uint4 &v, int k, float scale = 1.0f) { return eight_of(word_of(v, 2 * k), word_of(v, 2 * k + 1), scale); }
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t c) { return ((c & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u; } // bit 7 of the bytes that are NaN
+__device__ __forceinline__ uint4 without_nan(const uint4 &c) {
+    return make_uint4(c.x & ~((nan_bytes(c.x) >> 7) * 255), c.y & ~((nan_bytes(c.y) >> 7) * 255), c.z & ~((nan_bytes(c.z) >> 7) * 255), c.w & ~((nan_bytes(c.w) >> 7) * 255));
+}
 // over the four lanes that share a row
 __device__ __forceinline__ float quads_max(float x) {
     x = fmaxf(x, __shfl_xor(x, 16));
@@ -86,6 +92,7 @@ __device__ __forceinline__ float quads_sum(float x) {
 template <class T, int NL, int RT, bool ROWS>
 __global__ __launch_bounds__(64 * kWavesOfAttention, NL * RT > 2 ? 1 : 2) void cache_attention_kernel(CacheAttentionPlan p) {
     constexpr int kPieces = sizeof(T) == 4 ? 2 : 1, NV = 4 * NL, kSteps = 2 * NL;
+    constexpr bool kTotals = kPieces == 1; // the instruction adds to the totals itself
     const Cache8 &c = p.cache;
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, quad = lane >> 4;
     uint32_t id = blockIdx.x;
@@ -183,50 +190,47 @@ __global__ __launch_bounds__(64 * kWavesOfAttention, NL * RT > 2 ? 1 : 2) void c
     const uint32_t nb = c.capacity >> c.block_log2;
     const uint8_t *const keys = c.k_codes + (uint64_t)bg * c.capacity * c.dim, *const values = c.v_codes + (uint64_t)bg * c.capacity * c.vdim;
     const float *const k_scale = c.k_scale + (uint64_t)bg * nb, *const v_scale = c.v_scale + (uint64_t)bg * nb;
-    uint4 k_next[4][NL], k_now[4][NL], v_now[NV];
-    float ks_next = 0.0f, vs_next = 0.0f;
-    // (Addresses stay within the cache: a tile may reach behind its capacity, where no row sees anything.)
+    uint4 k_now[4][NL], v_now[NV];
+    float ks_now = 0.0f, vs_now = 0.0f;
+    // (Addresses stay within the cache: a tile may reach behind its capacity, where no row sees anything; behind dim the query is zero
+    // and any code of the same key will do, behind vdim nothing is made of the totals.)
     auto ask_keys = [&](uint32_t t) {
 #pragma unroll
         for (int kt = 0; kt < 4; kt++) {
             const uint32_t at = min(t * kTile + (col >> 2) * 16 + kt * 4 + (col & 3), c.capacity - 1);
 #pragma unroll
             for (int l = 0; l < NL; l++) {
-                const uint32_t d = l * 64 + quad * 16; // behind dim the query is zero: any code of the same key will do
-                k_next[kt][l] = *reinterpret_cast<const uint4 *>(keys + (uint64_t)at * c.dim + (d < c.dim ? d : 0));
+                const uint32_t d = l * 64 + quad * 16;
+                k_now[kt][l] = *reinterpret_cast<const uint4 *>(keys + (uint64_t)at * c.dim + (d < c.dim ? d : 0));
             }
         }
-        const uint32_t blk = min((t * kTile + quad * 16) >> c.block_log2, nb - 1);
-        ks_next = k_scale[blk];
-        vs_next = v_scale[blk];
+        ks_now = k_scale[min((t * kTile + quad * 16) >> c.block_log2, nb - 1)];
     };
     auto ask_values = [&](uint32_t t) {
         const uint32_t at = t * kTile + quad * 16, blk = min(at >> c.block_log2, nb - 1);
         const uint8_t *src = values + (((uint64_t)blk * c.vdim + col) << c.block_log2) + (at & ((1u << c.block_log2) - 1));
 #pragma unroll
-        for (int v = 0; v < NV; v++)
-            if (v * 16 < (int)c.vdim) v_now[v] = *reinterpret_cast<const uint4 *>(src + ((uint64_t)(v * 16) << c.block_log2));
+        for (int v = 0; v < NV; v++) v_now[v] = *reinterpret_cast<const uint4 *>(src + ((uint64_t)min(v * 16u, c.vdim - 16) << c.block_log2));
+        vs_now = v_scale[blk];
     };
-    float4v total[RT][NV];
-    float maximum[RT], sum[RT];
+    // Totals: sums of weight * value in units of 2^unit.  sums: of the weights, by the same instruction from ones.
+    float4v total[RT][NV], sums[RT];
+    float maximum[RT];
+    int unit = kLowestScale;
+    const half8v ones = {1, 1, 1, 1, 1, 1, 1, 1};
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
         maximum[rt] = kNoMaximum;
-        sum[rt] = 0.0f;
+        sums[rt] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int v = 0; v < NV; v++) total[rt][v] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
     }
-#pragma unroll
-    for (int v = 0; v < NV; v++) v_now[v] = make_uint4(0, 0, 0, 0);
-    if (tile < end_tile) ask_keys(tile);
-    for (; tile < end_tile; tile += kStride) {
-#pragma unroll
-        for (int kt = 0; kt < 4; kt++)
-#pragma unroll
-            for (int l = 0; l < NL; l++) k_now[kt][l] = k_next[kt][l];
-        const float ks = ks_next, vs = vs_next;
+    if (tile < end_tile) {
+        ask_keys(tile);
         ask_values(tile);
-        if (tile + kStride < end_tile) ask_keys(tile + kStride);
+    }
+    for (; tile < end_tile; tile += kStride) {
+        const bool more = tile + kStride < end_tile;
         const int at0 = (int)(tile * kTile), mine = at0 + (int)quad * 16; // the tile's first position, the lane's
         const bool masked = at0 < all_from || at0 + (int)kTile - 1 > all_to;
         // scores^T
@@ -246,6 +250,8 @@ __global__ __launch_bounds__(64 * kWavesOfAttention, NL * RT > 2 ? 1 : 2) void c
                 score[rt][kt] = s;
             }
         }
+        const float ks = ks_now;
+        if (more) ask_keys(tile + kStride); // (into the registers that the products have read)
         auto sees = [&](int rt, int i) { return mine + i >= begin[rt] && mine + i <= last[rt]; }; // i: of the lane's 16 positions
         // the maxima
         float factor[RT], largest[RT];
@@ -269,24 +275,21 @@ __global__ __launch_bounds__(64 * kWavesOfAttention, NL * RT > 2 ? 1 : 2) void c
             for (int rt = 0; rt < RT; rt++) {
                 const float m = fmaxf(maximum[rt], quads_max(largest[rt])), down = __builtin_amdgcn_exp2f(maximum[rt] - m);
                 maximum[rt] = m;
-                sum[rt] *= down;
+                sums[rt] *= down;
 #pragma unroll
                 for (int v = 0; v < NV; v++) total[rt][v] *= down;
             }
         }
-        // the weights
-        float weight[RT][16];
+        // the weights (in the scores' registers)
 #pragma unroll
         for (int rt = 0; rt < RT; rt++) {
             const float above = 8.0f - maximum[rt];
 #pragma unroll
-            for (int i = 0; i < 16; i++) weight[rt][i] = __builtin_amdgcn_exp2f(fmaf(score[rt][i / 4][i % 4], factor[rt], above));
+            for (int i = 0; i < 16; i++) score[rt][i / 4][i % 4] = __builtin_amdgcn_exp2f(fmaf(score[rt][i / 4][i % 4], factor[rt], above));
             if (masked) {
 #pragma unroll
-                for (int i = 0; i < 16; i++) weight[rt][i] = sees(rt, i) ? weight[rt][i] : 0.0f;
+                for (int i = 0; i < 16; i++) score[rt][i / 4][i % 4] = sees(rt, i) ? score[rt][i / 4][i % 4] : 0.0f;
             }
-#pragma unroll
-            for (int i = 0; i < 16; i++) sum[rt] += weight[rt][i];
         }
         // NaN among the values of a tile that not every row sees whole
         if (masked) {
@@ -296,82 +299,96 @@ __global__ __launch_bounds__(64 * kWavesOfAttention, NL * RT > 2 ? 1 : 2) void c
 #pragma unroll
                 for (int w = 0; w < 4; w++) found |= nan_bytes(word_of(v_now[v], w));
             if (__any(found != 0)) {
-                half8v seen[RT][2];
 #pragma unroll
-                for (int rt = 0; rt < RT; rt++)
+                for (int rt = 0; rt < RT; rt++) {
+                    half8v seen[2];
 #pragma unroll
-                    for (int i = 0; i < 16; i++) seen[rt][i / 8][i % 8] = sees(rt, i) ? (_Float16)1.0f : (_Float16)0.0f;
+                    for (int i = 0; i < 16; i++) seen[i / 8][i % 8] = sees(rt, i) ? (_Float16)1.0f : (_Float16)0.0f;
 #pragma unroll
-                for (int v = 0; v < NV; v++) {
-                    uint32_t x[4], one[4]; // the codes without NaN; the code of 1 where one was
-#pragma unroll
-                    for (int w = 0; w < 4; w++) {
-                        const uint32_t bytes = (nan_bytes(word_of(v_now[v], w)) >> 7) * 255;
-                        x[w] = word_of(v_now[v], w) & ~bytes;
-                        one[w] = bytes & 0x38383838u;
-                    }
-                    v_now[v] = make_uint4(x[0], x[1], x[2], x[3]);
-#pragma unroll
-                    for (int rt = 0; rt < RT; rt++) {
+                    for (int v = 0; v < NV; v++) {
                         float4v n = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                        for (int st = 0; st < 2; st++) n = __builtin_amdgcn_mfma_f32_16x16x32_f16(eight_of(one[2 * st], one[2 * st + 1]), seen[rt][st], n, 0, 0, 0);
+                        for (int st = 0; st < 2; st++) { // from the code of 1 where a NaN is
+                            const uint32_t lo = (nan_bytes(word_of(v_now[v], 2 * st)) >> 7) * 0x38, hi = (nan_bytes(word_of(v_now[v], 2 * st + 1)) >> 7) * 0x38;
+                            n = __builtin_amdgcn_mfma_f32_16x16x32_f16(eight_of(lo, hi, 1.0f), seen[st], n, 0, 0, 0);
+                        }
 #pragma unroll
                         for (int i = 0; i < 4; i++) total[rt][v][i] = n[i] > 0.0f ? NAN : total[rt][v][i];
                     }
                 }
+#pragma unroll
+                for (int v = 0; v < NV; v++) v_now[v] = without_nan(v_now[v]);
             }
         }
-        // the value blocks' scales
-        int e = scale_exponent(vs), largest_e = e;
-        uint32_t passes = 1;
-        float block_factor = 1.0f;
+        // the value blocks' scales: of the lane's block, the largest and the smallest of the tile
+        int e = scale_exponent(vs_now), largest_e, smallest_e;
         if (c.block_log2 < 6) {
-            const int lowest = -1000;
             const bool seen = mine + 15 >= any_from && mine <= any_to; // (a block that no row sees counts for nothing: its scale may be anything)
-            largest_e = quads_max(seen ? e : lowest);
-            const int smallest_e = -quads_max(seen ? -e : lowest);
+            const int none = -1000;
+            largest_e = quads_max(seen ? e : none);
+            smallest_e = -quads_max(seen ? -e : none);
+            if (largest_e == none) largest_e = smallest_e = kLowestScale;
             e = seen ? e : largest_e;
-            if (largest_e == lowest) e = largest_e = 0;
-            else if (largest_e - smallest_e > 8) passes = 4;
-            block_factor = power_of_two(max(e - largest_e, -126));
+        } else {
+            largest_e = smallest_e = e;
         }
-        for (uint32_t pass = 0; pass < passes; pass++) { // (the same for all lanes of a wave)
-            float out_factor = power_of_two(largest_e);
-            if (passes > 1) {
-                block_factor = quad == pass ? 1.0f : 0.0f;
-                out_factor = power_of_two(__shfl(e, (int)(pass * 16)));
+        largest_e = __builtin_amdgcn_readfirstlane(largest_e);
+        smallest_e = __builtin_amdgcn_readfirstlane(smallest_e);
+        half8v w[RT][kPieces][2];
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const float x = score[rt][i / 4][i % 4];
+                const _Float16 h = (_Float16)x;
+                w[rt][0][i / 8][i % 8] = h;
+                if (kPieces == 2) w[rt][kPieces - 1][i / 8][i % 8] = (_Float16)(x - (float)h);
             }
-            half8v w[RT][kPieces][2];
+            float4v s = kTotals ? sums[rt] : float4v{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int rt = 0; rt < RT; rt++)
+            for (int piece = kPieces - 1; piece >= 0; piece--)
 #pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    float x = weight[rt][i];
-                    if (c.block_log2 < 6) x = passes > 1 && block_factor == 0.0f ? 0.0f : x * block_factor; // (NaN stays in its block)
-                    const _Float16 h = (_Float16)x;
-                    w[rt][0][i / 8][i % 8] = h;
-                    if (kPieces == 2) w[rt][kPieces - 1][i / 8][i % 8] = (_Float16)(x - (float)h);
-                }
+                for (int st = 0; st < 2; st++) s = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, w[rt][piece][st], s, 0, 0, 0);
+            sums[rt] = kTotals ? s : sums[rt] + s;
+        }
+        const int passes = largest_e - smallest_e > kExact ? 4 : 1; // (the same for all lanes of a wave)
+        for (int pass = 0; pass < passes; pass++) {
+            const int wanted = passes > 1 ? __builtin_amdgcn_readlane(e, pass * 16) : largest_e;
+            if (wanted > unit || wanted < unit - kExact) { // the totals in units of this scale
+                const int to = max(wanted, unit - kMostDown);
+                const float by = power_of_two(max(unit - to, -126));
+                unit = to;
+#pragma unroll
+                for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+                    for (int v = 0; v < NV; v++) total[rt][v] *= by;
+            }
+            const float scale = passes == 1 || (int)quad == pass ? power_of_two(max(e - unit, -126)) : 0.0f;
 #pragma unroll
             for (int v = 0; v < NV; v++) {
-                if (v * 16 >= (int)c.vdim) continue;
-                const half8v a[2] = {eight_of(v_now[v], 0), eight_of(v_now[v], 1)};
+                half8v a[2];
+#pragma unroll
+                for (int st = 0; st < 2; st++) a[st] = eight_of(v_now[v], st, scale);
 #pragma unroll
                 for (int rt = 0; rt < RT; rt++) {
-                    float4v s = {0.0f, 0.0f, 0.0f, 0.0f};
+                    float4v s = kTotals ? total[rt][v] : float4v{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                     for (int piece = kPieces - 1; piece >= 0; piece--)
 #pragma unroll
                         for (int st = 0; st < 2; st++) s = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[st], w[rt][piece][st], s, 0, 0, 0);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) total[rt][v][i] = fmaf(s[i], out_factor, total[rt][v][i]);
+                    total[rt][v] = kTotals ? s : total[rt][v] + s;
                 }
             }
         }
+        if (more) ask_values(tile + kStride);
     }
+    float sum[RT];
 #pragma unroll
-    for (int rt = 0; rt < RT; rt++) sum[rt] = quads_sum(sum[rt]);
+    for (int rt = 0; rt < RT; rt++) {
+        sum[rt] = sums[rt][0];
+#pragma unroll
+        for (int v = 0; v < NV; v++) total[rt][v] *= power_of_two(unit);
+    }
 
     // ---- the waves' results together: of two and two, then of the last two
     if (!ROWS) {
