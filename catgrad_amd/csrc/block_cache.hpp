@@ -11,8 +11,11 @@ struct LaunchOn {
     LaunchQueue *queue = nullptr;
     hipStream_t stream = nullptr;
     template <class... P, class... A> int operator()(const char *what, void (*kernel)(P...), dim3 grid, dim3 block, A &&...a) const {
-        if (queue) launch_kernel(kernel, grid, block, 0, *queue, std::forward<A>(a)...);
-        else hipLaunchKernelGGL(kernel, grid, block, 0, stream, std::forward<A>(a)...);
+        return with_lds(what, kernel, grid, block, 0, std::forward<A>(a)...);
+    }
+    template <class... P, class... A> int with_lds(const char *what, void (*kernel)(P...), dim3 grid, dim3 block, size_t lds, A &&...a) const {
+        if (queue) launch_kernel(kernel, grid, block, lds, *queue, std::forward<A>(a)...);
+        else hipLaunchKernelGGL(kernel, grid, block, lds, stream, std::forward<A>(a)...);
         const hipError_t e = hipGetLastError();
         return e == hipSuccess ? CG_OK : hip_fail(e, what);
     }

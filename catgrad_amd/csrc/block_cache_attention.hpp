@@ -87,159 +87,125 @@ __device__ __forceinline__ float quads_sum(float x) {
     return x + __shfl_xor(x, 32);
 }
 
-// ROWS: every wave of a workgroup has rows of its own and walks all of their tiles; else the waves have the same rows, take the
-// tiles in turns and add their results up in LDS.  RT: 16-row groups of a wave.  NL: 64-channel pieces of a head.
-template <class T, int NL, int RT, bool ROWS>
-__global__ __launch_bounds__(64 * kWavesOfAttention, NL * RT > 2 ? 1 : 2) void cache_attention_kernel(CacheAttentionPlan p) {
-    constexpr int kPieces = sizeof(T) == 4 ? 2 : 1, NV = 4 * NL, kSteps = 2 * NL;
-    constexpr bool kTotals = kPieces == 1; // the instruction adds to the totals itself
-    const Cache8 &c = p.cache;
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, quad = lane >> 4;
-    uint32_t id = blockIdx.x;
-    const uint32_t bg = id % p.bgs;
-    id /= p.bgs;
-    const uint32_t split = id % p.splits, row_block = p.row_blocks - 1 - id / p.splits; // (the longest rows first)
-    const uint32_t b = bg / c.kv_heads, g = bg - b * c.kv_heads;
-    const uint64_t held = p.batch.held_by(b);
-    const uint32_t R = p.batch.count_of(b) * p.rep, group = (ROWS ? kWavesOfAttention : 1) * 16 * RT, group0 = row_block * group;
-    if (group0 >= R) return;
-    const KeyRange range = key_range(p, held, group0 / p.rep, (min(group0 + group, R) - 1) / p.rep);
-    if (split >= range.parts) return;
-    uint32_t tile = range.first_tile + split * range.each, end_tile = min(tile + range.each, range.end_tile);
-    const uint32_t row0 = group0 + (ROWS ? wave * 16 * RT : 0);
-    if (ROWS) {
-        if (row0 >= R) return;
-        CacheAttentionPlan whole = p;
-        whole.splits = 1;
-        const KeyRange mine = key_range(whole, held, row0 / p.rep, (min(row0 + 16 * RT, R) - 1) / p.rep);
-        tile = max(tile, mine.first_tile);
-        end_tile = min(end_tile, mine.end_tile);
-    } else {
-        tile += wave;
-    }
-    constexpr uint32_t kStride = ROWS ? 1 : kWavesOfAttention;
+// What a wave knows of its rows, and does with a tile.  RT: 16-row groups; NL: 64-channel pieces of a head.
+template <class T, int NL, int RT> struct AttentionWave {
+    static constexpr int kPieces = sizeof(T) == 4 ? 2 : 1, NV = 4 * NL, kSteps = 2 * NL;
+    static constexpr bool kTotals = kPieces == 1; // the instruction adds to the totals itself
 
-    // ---- the rows: their queries, and which positions they see
+    const CacheAttentionPlan &p;
+    const uint32_t lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
+    uint32_t b, g, row0, R;
     half8v q[RT][kPieces][kSteps];
     float row_factor[RT];
-    int last[RT], begin[RT]; // positions begin .. last; none: last < begin
-    int64_t row_token[RT];   // (for the results)
-    const bool whole_q = reinterpret_cast<uintptr_t>(p.q) % 16 == 0 && p.q_pitch * sizeof(T) % 16 == 0;
-#pragma unroll
-    for (int rt = 0; rt < RT; rt++) {
-        const uint32_t r = row0 + rt * 16 + col, rr = min(r, R - 1), s = rr / p.rep, head = g * p.rep + rr - s * p.rep;
-        row_token[rt] = (int64_t)b * p.batch.tokens + s;
-        const uint64_t at = held + s; // its position
-        last[rt] = r < R ? (int)min(at, (uint64_t)c.capacity - 1) : -1;
-        begin[rt] = p.window && at + 1 > p.window ? (int)min(at + 1 - p.window, (uint64_t)c.capacity) : 0;
-        const T *src = static_cast<const T *>(p.q) + row_token[rt] * p.q_pitch + head * c.dim;
-        float x[NL][16], size = 0.0f, bad = 0.0f;
-#pragma unroll
-        for (int l = 0; l < NL; l++) {
-            const uint32_t d = l * 64 + quad * 16;
-            if (d < c.dim) {
-                load_elements<T, 16>(src + d, whole_q, x[l]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 16; i++) x[l][i] = 0.0f;
-            }
-#pragma unroll
-            for (int i = 0; i < 16; i++) {
-                size = fmaxf(size, fabsf(x[l][i]));
-                bad += x[l][i] * 0.0f;
-            }
-        }
-        size = quads_max(size);
-        bad = quads_sum(bad); // 0, or NaN where a value is not finite: then so are the row's scores
-        const int e = bad == 0.0f && size > 0.0f ? __builtin_amdgcn_frexp_expf(size) : 0;
-        row_factor[rt] = bad == 0.0f ? ldexpf(fabsf(p.scale) * 1.44269504088896341f, e - 8) : bad;
-        const float sign = p.scale < 0.0f ? -1.0f : 1.0f;
-#pragma unroll
-        for (int l = 0; l < NL; l++)
-#pragma unroll
-            for (int i = 0; i < 16; i++) {
-                const float y = bad == 0.0f ? ldexpf(x[l][i], 8 - e) * sign : 0.0f;
-                const _Float16 h = (_Float16)y;
-                q[rt][0][2 * l + i / 8][i % 8] = h;
-                if (kPieces == 2) q[rt][kPieces - 1][2 * l + i / 8][i % 8] = (_Float16)(y - (float)h);
-            }
-    }
-    // positions that all of the wave's rows see, and those that any does
-    int all_from = 0, all_to = 0x7FFFFFFF, any_from = 0x7FFFFFFF, any_to = -1;
-#pragma unroll
-    for (int rt = 0; rt < RT; rt++)
-        if (last[rt] >= 0) {
-            all_from = max(all_from, begin[rt]);
-            all_to = min(all_to, last[rt]);
-            any_from = min(any_from, begin[rt]);
-            any_to = max(any_to, last[rt]);
-        }
-#pragma unroll
-    for (int o = 1; o < 16; o <<= 1) {
-        all_from = max(all_from, __shfl_xor(all_from, o));
-        all_to = min(all_to, __shfl_xor(all_to, o));
-        any_from = min(any_from, __shfl_xor(any_from, o));
-        any_to = max(any_to, __shfl_xor(any_to, o));
-    }
-    all_from = __builtin_amdgcn_readfirstlane(all_from);
-    all_to = __builtin_amdgcn_readfirstlane(all_to);
-    any_from = __builtin_amdgcn_readfirstlane(any_from);
-    any_to = __builtin_amdgcn_readfirstlane(any_to);
-
-    // ---- the tiles
-    const uint32_t nb = c.capacity >> c.block_log2;
-    const uint8_t *const keys = c.k_codes + (uint64_t)bg * c.capacity * c.dim, *const values = c.v_codes + (uint64_t)bg * c.capacity * c.vdim;
-    const float *const k_scale = c.k_scale + (uint64_t)bg * nb, *const v_scale = c.v_scale + (uint64_t)bg * nb;
-    uint4 k_now[4][NL], v_now[NV];
-    float ks_now = 0.0f, vs_now = 0.0f;
-    // (Addresses stay within the cache: a tile may reach behind its capacity, where no row sees anything; behind dim the query is zero
-    // and any code of the same key will do, behind vdim nothing is made of the totals.)
-    auto ask_keys = [&](uint32_t t) {
-#pragma unroll
-        for (int kt = 0; kt < 4; kt++) {
-            const uint32_t at = min(t * kTile + (col >> 2) * 16 + kt * 4 + (col & 3), c.capacity - 1);
-#pragma unroll
-            for (int l = 0; l < NL; l++) {
-                const uint32_t d = l * 64 + quad * 16;
-                k_now[kt][l] = *reinterpret_cast<const uint4 *>(keys + (uint64_t)at * c.dim + (d < c.dim ? d : 0));
-            }
-        }
-        ks_now = k_scale[min((t * kTile + quad * 16) >> c.block_log2, nb - 1)];
-    };
-    auto ask_values = [&](uint32_t t) {
-        const uint32_t at = t * kTile + quad * 16, blk = min(at >> c.block_log2, nb - 1);
-        const uint8_t *src = values + (((uint64_t)blk * c.vdim + col) << c.block_log2) + (at & ((1u << c.block_log2) - 1));
-#pragma unroll
-        for (int v = 0; v < NV; v++) v_now[v] = *reinterpret_cast<const uint4 *>(src + ((uint64_t)min(v * 16u, c.vdim - 16) << c.block_log2));
-        vs_now = v_scale[blk];
-    };
+    int last[RT], begin[RT]; // positions begin .. last that the lane's rows see; none: last < begin
+    int all_from, all_to, any_from, any_to; // positions that all of the wave's rows see, that any does
     // Totals: sums of weight * value in units of 2^unit.  sums: of the weights, by the same instruction from ones.
     float4v total[RT][NV], sums[RT];
     float maximum[RT];
     int unit = kLowestScale;
-    const half8v ones = {1, 1, 1, 1, 1, 1, 1, 1};
+    // of the tile at hand
+    float4v score[RT][4];
+    int mine;    // the lane's first position
+    bool masked; // not all rows see all of it
+
+    __device__ __forceinline__ AttentionWave(const CacheAttentionPlan &plan) : p(plan) {}
+    __device__ __forceinline__ int64_t token_of(int rt) const { return (int64_t)b * p.batch.tokens + min(row0 + rt * 16 + col, R - 1) / p.rep; }
+
+    // The queries of rows row0 .. of a pair's R rows.
+    __device__ __forceinline__ void begin_rows(uint64_t held) {
+        const Cache8 &c = p.cache;
+        const bool whole_q = reinterpret_cast<uintptr_t>(p.q) % 16 == 0 && p.q_pitch * sizeof(T) % 16 == 0;
+        all_from = 0, all_to = 0x7FFFFFFF, any_from = 0x7FFFFFFF, any_to = -1;
 #pragma unroll
-    for (int rt = 0; rt < RT; rt++) {
-        maximum[rt] = kNoMaximum;
-        sums[rt] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int rt = 0; rt < RT; rt++) {
+            const uint32_t r = row0 + rt * 16 + col, rr = min(r, R - 1), s = rr / p.rep, head = g * p.rep + rr - s * p.rep;
+            const uint64_t at = held + s; // its position
+            last[rt] = r < R ? (int)min(at, (uint64_t)c.capacity - 1) : -1;
+            begin[rt] = p.window && at + 1 > p.window ? (int)min(at + 1 - p.window, (uint64_t)c.capacity) : 0;
+            const T *src = static_cast<const T *>(p.q) + token_of(rt) * p.q_pitch + head * c.dim;
+            float x[NL][16], size = 0.0f, bad = 0.0f;
 #pragma unroll
-        for (int v = 0; v < NV; v++) total[rt][v] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int l = 0; l < NL; l++) {
+                const uint32_t d = l * 64 + quad * 16;
+                if (d < c.dim) {
+                    load_elements<T, 16>(src + d, whole_q, x[l]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16; i++) x[l][i] = 0.0f;
+                }
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    size = fmaxf(size, fabsf(x[l][i]));
+                    bad += x[l][i] * 0.0f;
+                }
+            }
+            size = quads_max(size);
+            bad = quads_sum(bad); // 0, or NaN where a value is not finite: then so are the row's scores
+            const int e = bad == 0.0f && size > 0.0f ? __builtin_amdgcn_frexp_expf(size) : 0;
+            row_factor[rt] = bad == 0.0f ? ldexpf(fabsf(p.scale) * 1.44269504088896341f, e - 8) : bad;
+            const float sign = p.scale < 0.0f ? -1.0f : 1.0f;
+#pragma unroll
+            for (int l = 0; l < NL; l++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const float y = bad == 0.0f ? ldexpf(x[l][i], 8 - e) * sign : 0.0f;
+                    const _Float16 h = (_Float16)y;
+                    q[rt][0][2 * l + i / 8][i % 8] = h;
+                    if (kPieces == 2) q[rt][kPieces - 1][2 * l + i / 8][i % 8] = (_Float16)(y - (float)h);
+                }
+            if (last[rt] >= 0) {
+                all_from = max(all_from, begin[rt]);
+                all_to = min(all_to, last[rt]);
+                any_from = min(any_from, begin[rt]);
+                any_to = max(any_to, last[rt]);
+            }
+            maximum[rt] = kNoMaximum;
+            sums[rt] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int v = 0; v < NV; v++) total[rt][v] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) {
+            all_from = max(all_from, __shfl_xor(all_from, o));
+            all_to = min(all_to, __shfl_xor(all_to, o));
+            any_from = min(any_from, __shfl_xor(any_from, o));
+            any_to = max(any_to, __shfl_xor(any_to, o));
+        }
+        all_from = __builtin_amdgcn_readfirstlane(all_from);
+        all_to = __builtin_amdgcn_readfirstlane(all_to);
+        any_from = __builtin_amdgcn_readfirstlane(any_from);
+        any_to = __builtin_amdgcn_readfirstlane(any_to);
     }
-    if (tile < end_tile) {
-        ask_keys(tile);
-        ask_values(tile);
+
+    // Where a tile's codes lie: those of position row kt, channel piece l, and of channel group v.  (Addresses stay within the cache: a tile
+    // may reach behind its capacity, where no row sees anything; behind dim the query is zero and any code of the same key will do, behind vdim
+    // nothing is made of the totals.)
+    __device__ __forceinline__ const uint4 *key_codes(const uint8_t *keys, uint32_t t, int kt, int l) const {
+        const uint32_t at = min(t * kTile + (col >> 2) * 16 + kt * 4 + (col & 3), p.cache.capacity - 1), d = l * 64 + quad * 16;
+        return reinterpret_cast<const uint4 *>(keys + (uint64_t)at * p.cache.dim + (d < p.cache.dim ? d : 0));
     }
-    for (; tile < end_tile; tile += kStride) {
-        const bool more = tile + kStride < end_tile;
-        const int at0 = (int)(tile * kTile), mine = at0 + (int)quad * 16; // the tile's first position, the lane's
-        const bool masked = at0 < all_from || at0 + (int)kTile - 1 > all_to;
-        // scores^T
-        float4v score[RT][4];
+    __device__ __forceinline__ uint32_t block_of(uint32_t t) const { return min((t * kTile + quad * 16) >> p.cache.block_log2, (p.cache.capacity >> p.cache.block_log2) - 1); }
+    __device__ __forceinline__ const uint4 *value_codes(const uint8_t *values, uint32_t t, int v) const {
+        const uint32_t n = p.cache.block_log2, at = (t * kTile + quad * 16) & ((1u << n) - 1);
+        return reinterpret_cast<const uint4 *>(values + (((uint64_t)block_of(t) * p.cache.vdim + min(v * 16u, p.cache.vdim - 16) + col) << n) + at);
+    }
+
+    __device__ __forceinline__ bool sees(int rt, int i) const { return mine + i >= begin[rt] && mine + i <= last[rt]; } // i: of the lane's 16 positions
+
+    // scores^T; keys(kt, l): the codes
+    template <class K> __device__ __forceinline__ void scores(uint32_t t, K &&keys) {
+        const int at = (int)(t * kTile);
+        mine = at + (int)quad * 16;
+        masked = at < all_from || at + (int)kTile - 1 > all_to;
 #pragma unroll
         for (int kt = 0; kt < 4; kt++) {
             half8v a[kSteps];
 #pragma unroll
-            for (int st = 0; st < kSteps; st++) a[st] = eight_of(k_now[kt][st / 2], st % 2);
+            for (int l = 0; l < NL; l++) {
+                const uint4 codes = keys(kt, l);
+                a[2 * l] = eight_of(codes, 0);
+                a[2 * l + 1] = eight_of(codes, 1);
+            }
 #pragma unroll
             for (int rt = 0; rt < RT; rt++) {
                 float4v s = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -250,10 +216,10 @@ __global__ __launch_bounds__(64 * kWavesOfAttention, NL * RT > 2 ? 1 : 2) void c
                 score[rt][kt] = s;
             }
         }
-        const float ks = ks_now;
-        if (more) ask_keys(tile + kStride); // (into the registers that the products have read)
-        auto sees = [&](int rt, int i) { return mine + i >= begin[rt] && mine + i <= last[rt]; }; // i: of the lane's 16 positions
-        // the maxima
+    }
+
+    // The scores become weights; ks: the scale of the lane's block.
+    __device__ __forceinline__ void weigh(float ks) {
         float factor[RT], largest[RT];
         bool moves = false;
 #pragma unroll
@@ -280,7 +246,6 @@ __global__ __launch_bounds__(64 * kWavesOfAttention, NL * RT > 2 ? 1 : 2) void c
                 for (int v = 0; v < NV; v++) total[rt][v] *= down;
             }
         }
-        // the weights (in the scores' registers)
 #pragma unroll
         for (int rt = 0; rt < RT; rt++) {
             const float above = 8.0f - maximum[rt];
@@ -291,13 +256,19 @@ __global__ __launch_bounds__(64 * kWavesOfAttention, NL * RT > 2 ? 1 : 2) void c
                 for (int i = 0; i < 16; i++) score[rt][i / 4][i % 4] = sees(rt, i) ? score[rt][i / 4][i % 4] : 0.0f;
             }
         }
+    }
+
+    // out^T += V^T weights^T; values(v): the codes, without NaN from the call of clean() on; vs: the scale of the lane's block
+    template <class V, class C> __device__ __forceinline__ void products(float vs, V &&values, C &&clean) {
         // NaN among the values of a tile that not every row sees whole
         if (masked) {
             uint32_t found = 0;
 #pragma unroll
-            for (int v = 0; v < NV; v++)
-#pragma unroll
-                for (int w = 0; w < 4; w++) found |= nan_bytes(word_of(v_now[v], w));
+            for (int v = 0; v < NV; v++) {
+                const uint4 codes = values(v);
+                found |= nan_bytes(codes.x) | nan_bytes(codes.y) | nan_bytes(codes.z) | nan_bytes(codes.w);
+            }
+            asm volatile("" ::: "memory"); // (codes in LDS are read where they are used, not all of them in front)
             if (__any(found != 0)) {
 #pragma unroll
                 for (int rt = 0; rt < RT; rt++) {
@@ -306,23 +277,24 @@ __global__ __launch_bounds__(64 * kWavesOfAttention, NL * RT > 2 ? 1 : 2) void c
                     for (int i = 0; i < 16; i++) seen[i / 8][i % 8] = sees(rt, i) ? (_Float16)1.0f : (_Float16)0.0f;
 #pragma unroll
                     for (int v = 0; v < NV; v++) {
+                        const uint4 codes = values(v);
                         float4v n = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                         for (int st = 0; st < 2; st++) { // from the code of 1 where a NaN is
-                            const uint32_t lo = (nan_bytes(word_of(v_now[v], 2 * st)) >> 7) * 0x38, hi = (nan_bytes(word_of(v_now[v], 2 * st + 1)) >> 7) * 0x38;
+                            const uint32_t lo = (nan_bytes(word_of(codes, 2 * st)) >> 7) * 0x38, hi = (nan_bytes(word_of(codes, 2 * st + 1)) >> 7) * 0x38;
                             n = __builtin_amdgcn_mfma_f32_16x16x32_f16(eight_of(lo, hi, 1.0f), seen[st], n, 0, 0, 0);
                         }
 #pragma unroll
                         for (int i = 0; i < 4; i++) total[rt][v][i] = n[i] > 0.0f ? NAN : total[rt][v][i];
+                        __builtin_amdgcn_sched_barrier(0); // (few do this: in few registers)
                     }
                 }
-#pragma unroll
-                for (int v = 0; v < NV; v++) v_now[v] = without_nan(v_now[v]);
+                clean();
             }
         }
         // the value blocks' scales: of the lane's block, the largest and the smallest of the tile
-        int e = scale_exponent(vs_now), largest_e, smallest_e;
-        if (c.block_log2 < 6) {
+        int e = scale_exponent(vs), largest_e, smallest_e;
+        if (p.cache.block_log2 < 6) {
             const bool seen = mine + 15 >= any_from && mine <= any_to; // (a block that no row sees counts for nothing: its scale may be anything)
             const int none = -1000;
             largest_e = quads_max(seen ? e : none);
@@ -335,6 +307,7 @@ __global__ __launch_bounds__(64 * kWavesOfAttention, NL * RT > 2 ? 1 : 2) void c
         largest_e = __builtin_amdgcn_readfirstlane(largest_e);
         smallest_e = __builtin_amdgcn_readfirstlane(smallest_e);
         half8v w[RT][kPieces][2];
+        const half8v ones = {1, 1, 1, 1, 1, 1, 1, 1};
 #pragma unroll
         for (int rt = 0; rt < RT; rt++) {
 #pragma unroll
@@ -353,6 +326,7 @@ __global__ __launch_bounds__(64 * kWavesOfAttention, NL * RT > 2 ? 1 : 2) void c
         }
         const int passes = largest_e - smallest_e > kExact ? 4 : 1; // (the same for all lanes of a wave)
         for (int pass = 0; pass < passes; pass++) {
+            asm volatile("" ::: "memory");
             const int wanted = passes > 1 ? __builtin_amdgcn_readlane(e, pass * 16) : largest_e;
             if (wanted > unit || wanted < unit - kExact) { // the totals in units of this scale
                 const int to = max(wanted, unit - kMostDown);
@@ -366,9 +340,10 @@ __global__ __launch_bounds__(64 * kWavesOfAttention, NL * RT > 2 ? 1 : 2) void c
             const float scale = passes == 1 || (int)quad == pass ? power_of_two(max(e - unit, -126)) : 0.0f;
 #pragma unroll
             for (int v = 0; v < NV; v++) {
+                const uint4 codes = values(v);
                 half8v a[2];
 #pragma unroll
-                for (int st = 0; st < 2; st++) a[st] = eight_of(v_now[v], st, scale);
+                for (int st = 0; st < 2; st++) a[st] = eight_of(codes, st, scale);
 #pragma unroll
                 for (int rt = 0; rt < RT; rt++) {
                     float4v s = kTotals ? total[rt][v] : float4v{0.0f, 0.0f, 0.0f, 0.0f};
@@ -380,83 +355,229 @@ __global__ __launch_bounds__(64 * kWavesOfAttention, NL * RT > 2 ? 1 : 2) void c
                 }
             }
         }
-        if (more) ask_values(tile + kStride);
     }
-    float sum[RT];
+    __device__ __forceinline__ void end_tiles() {
 #pragma unroll
-    for (int rt = 0; rt < RT; rt++) {
-        sum[rt] = sums[rt][0];
+        for (int rt = 0; rt < RT; rt++)
 #pragma unroll
-        for (int v = 0; v < NV; v++) total[rt][v] *= power_of_two(unit);
+            for (int v = 0; v < NV; v++) total[rt][v] *= power_of_two(unit);
     }
 
-    // ---- the waves' results together: of two and two, then of the last two
-    if (!ROWS) {
-        __shared__ float4v shared_total[2][RT * NV][64];
-        __shared__ float2 shared_stats[2][RT][64];
+    // The rows' results, or those of one of their parts.
+    __device__ __forceinline__ void store(uint32_t parts, uint32_t split) const {
+        const Cache8 &c = p.cache;
 #pragma unroll
-        for (uint32_t half = 2; half >= 1; half /= 2) {
-            if (wave >= half && wave < 2 * half) {
+        for (int rt = 0; rt < RT; rt++) {
+            const uint32_t r = row0 + rt * 16 + col;
+            if (r >= R) continue;
+            const float sum = sums[rt][0];
+            if (parts == 1) {
+                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                const uint32_t head = g * p.rep + r % p.rep;
+                T *const dst = static_cast<T *>(p.out) + token_of(rt) * p.out_pitch + head * c.vdim + quad * 4;
+                const bool whole = reinterpret_cast<uintptr_t>(p.out) % (4 * sizeof(T)) == 0 && p.out_pitch % 4 == 0;
 #pragma unroll
-                for (int rt = 0; rt < RT; rt++) {
-                    shared_stats[wave - half][rt][lane] = make_float2(maximum[rt], sum[rt]);
-#pragma unroll
-                    for (int v = 0; v < NV; v++) shared_total[wave - half][rt * NV + v][lane] = total[rt][v];
+                for (int v = 0; v < NV; v++) {
+                    if (v * 16 >= (int)c.vdim) continue;
+                    const float y[4] = {total[rt][v][0] * inv, total[rt][v][1] * inv, total[rt][v][2] * inv, total[rt][v][3] * inv};
+                    store_elements<T, 4>(dst + v * 16, whole, y);
                 }
+            } else {
+                const uint64_t at = ((uint64_t)(b * c.kv_heads + g) * p.splits + split) * p.rows + r;
+                if (quad == 0) p.stats[at] = make_float2(maximum[rt], sum);
+                float *const dst = p.parts + at * c.vdim + quad * 4;
+#pragma unroll
+                for (int v = 0; v < NV; v++)
+                    if (v * 16 < (int)c.vdim) *reinterpret_cast<float4v *>(dst + v * 16) = total[rt][v];
             }
-            __syncthreads();
-            if (wave < half) {
-#pragma unroll
-                for (int rt = 0; rt < RT; rt++) {
-                    const float2 other = shared_stats[wave][rt][lane];
-                    const float m = fmaxf(maximum[rt], other.x), mine = __builtin_amdgcn_exp2f(maximum[rt] - m), its = __builtin_amdgcn_exp2f(other.x - m);
-                    maximum[rt] = m;
-                    sum[rt] = sum[rt] * mine + other.y * its;
-#pragma unroll
-                    for (int v = 0; v < NV; v++) total[rt][v] = total[rt][v] * mine + shared_total[wave][rt * NV + v][lane] * its;
-                }
-            }
-            __syncthreads();
-        }
-        if (wave > 0) return;
-    }
-#pragma unroll
-    for (int rt = 0; rt < RT; rt++) {
-        const uint32_t r = row0 + rt * 16 + col;
-        if (r >= R) continue;
-        if (range.parts == 1) {
-            const float inv = sum[rt] == 0.0f ? 0.0f : 1.0f / sum[rt];
-            const uint32_t head = g * p.rep + r % p.rep;
-            T *const dst = static_cast<T *>(p.out) + row_token[rt] * p.out_pitch + head * c.vdim + quad * 4;
-            const bool whole = reinterpret_cast<uintptr_t>(p.out) % (4 * sizeof(T)) == 0 && p.out_pitch % 4 == 0;
-#pragma unroll
-            for (int v = 0; v < NV; v++) {
-                if (v * 16 >= (int)c.vdim) continue;
-                const float y[4] = {total[rt][v][0] * inv, total[rt][v][1] * inv, total[rt][v][2] * inv, total[rt][v][3] * inv};
-                store_elements<T, 4>(dst + v * 16, whole, y);
-            }
-        } else {
-            const uint64_t at = ((uint64_t)bg * p.splits + split) * p.rows + r;
-            if (quad == 0) p.stats[at] = make_float2(maximum[rt], sum[rt]);
-            float *const dst = p.parts + at * c.vdim + quad * 4;
-#pragma unroll
-            for (int v = 0; v < NV; v++)
-                if (v * 16 < (int)c.vdim) *reinterpret_cast<float4v *>(dst + v * 16) = total[rt][v];
         }
     }
+};
+
+// Which rows and tiles a workgroup takes: `group` rows of a pair from group0 on, the tiles of part `split`.
+struct AttentionShare {
+    uint32_t bg, b, g, split, group0, R;
+    uint64_t held;
+    KeyRange range;
+    uint32_t tile, end_tile;
+    __device__ __forceinline__ bool find(const CacheAttentionPlan &p, uint32_t group) {
+        uint32_t id = blockIdx.x;
+        bg = id % p.bgs;
+        id /= p.bgs;
+        split = id % p.splits;
+        group0 = (p.row_blocks - 1 - id / p.splits) * group; // (the longest rows first)
+        b = bg / p.cache.kv_heads;
+        g = bg - b * p.cache.kv_heads;
+        held = p.batch.held_by(b);
+        R = p.batch.count_of(b) * p.rep;
+        if (group0 >= R) return false;
+        range = key_range(p, held, group0 / p.rep, (min(group0 + group, R) - 1) / p.rep);
+        if (split >= range.parts) return false;
+        tile = range.first_tile + split * range.each;
+        end_tile = min(tile + range.each, range.end_tile);
+        return true;
+    }
+};
+
+// Few rows: the waves of a workgroup have the same rows, take their tiles in turns, codes straight to registers, and add their results up
+// in LDS.  Bound by memory.
+template <class T, int NL, int RT> __global__ __launch_bounds__(64 * kWavesOfAttention, NL * RT > 2 ? 1 : 2) void cache_attention_kernel(CacheAttentionPlan p) {
+    typedef AttentionWave<T, NL, RT> Wave;
+    constexpr int NV = Wave::NV;
+    AttentionShare my;
+    if (!my.find(p, 16 * RT)) return;
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    Wave w(p);
+    w.b = my.b;
+    w.g = my.g;
+    w.R = my.R;
+    w.row0 = my.group0;
+    const Cache8 &c = p.cache;
+    const uint32_t nb = c.capacity >> c.block_log2;
+    const uint8_t *const keys = c.k_codes + (uint64_t)my.bg * c.capacity * c.dim, *const values = c.v_codes + (uint64_t)my.bg * c.capacity * c.vdim;
+    const float *const k_scale = c.k_scale + (uint64_t)my.bg * nb, *const v_scale = c.v_scale + (uint64_t)my.bg * nb;
+    uint4 k_now[4][NL], v_now[NV];
+    float ks_now = 0.0f, vs_now = 0.0f;
+    auto ask_keys = [&](uint32_t t) {
+#pragma unroll
+        for (int kt = 0; kt < 4; kt++)
+#pragma unroll
+            for (int l = 0; l < NL; l++) k_now[kt][l] = *w.key_codes(keys, t, kt, l);
+        ks_now = k_scale[w.block_of(t)];
+    };
+    auto ask_values = [&](uint32_t t) {
+#pragma unroll
+        for (int v = 0; v < NV; v++) v_now[v] = *w.value_codes(values, t, v);
+        vs_now = v_scale[w.block_of(t)];
+    };
+    uint32_t tile = my.tile + wave;
+    if (tile < my.end_tile) {
+        ask_keys(tile);
+        ask_values(tile);
+    }
+    w.begin_rows(my.held);
+    for (; tile < my.end_tile; tile += kWavesOfAttention) {
+        const bool more = tile + kWavesOfAttention < my.end_tile;
+        w.scores(tile, [&](int kt, int l) { return k_now[kt][l]; });
+        const float ks = ks_now;
+        if (more) ask_keys(tile + kWavesOfAttention); // (into the registers that the products have read)
+        w.weigh(ks);
+        w.products(vs_now, [&](int v) { return v_now[v]; },
+                   [&] {
+#pragma unroll
+                       for (int v = 0; v < NV; v++) v_now[v] = without_nan(v_now[v]);
+                   });
+        if (more) ask_values(tile + kWavesOfAttention);
+    }
+    w.end_tiles();
+    // the waves' results: of two and two, then of the last two
+    __shared__ float4v shared_total[2][RT * NV][64];
+    __shared__ float2 shared_stats[2][RT][64];
+#pragma unroll
+    for (uint32_t half = 2; half >= 1; half /= 2) {
+        if (wave >= half && wave < 2 * half) {
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++) {
+                shared_stats[wave - half][rt][lane] = make_float2(w.maximum[rt], w.sums[rt][0]);
+#pragma unroll
+                for (int v = 0; v < NV; v++) shared_total[wave - half][rt * NV + v][lane] = w.total[rt][v];
+            }
+        }
+        __syncthreads();
+        if (wave < half) {
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++) {
+                const float2 other = shared_stats[wave][rt][lane];
+                const float m = fmaxf(w.maximum[rt], other.x), mine = __builtin_amdgcn_exp2f(w.maximum[rt] - m), its = __builtin_amdgcn_exp2f(other.x - m);
+                w.maximum[rt] = m;
+                w.sums[rt][0] = w.sums[rt][0] * mine + other.y * its;
+#pragma unroll
+                for (int v = 0; v < NV; v++) w.total[rt][v] = w.total[rt][v] * mine + shared_total[wave][rt * NV + v][lane] * its;
+            }
+        }
+        __syncthreads();
+    }
+    if (wave == 0) w.store(my.range.parts, my.split);
+}
+
+// Many rows: every wave of a workgroup has rows of its own, and all walk the same tiles, whose codes come straight into LDS, a tile ahead, in
+// the order in which the lanes take them.  Bound by the vector instructions between the products (widening codes, weights).
+template <class T, int NL, int RT> __global__ __launch_bounds__(64 * kWavesOfAttention, 2) void cache_attention_rows_kernel(CacheAttentionPlan p) {
+    typedef AttentionWave<T, NL, RT> Wave;
+    typedef __attribute__((address_space(3))) char lds_char;
+    constexpr int kCodes = 8 * NL, kMine = kCodes / kWavesOfAttention; // 1 KB pieces of a tile, of which each wave asks for some
+    extern __shared__ float lds_dyn[];
+    lds_char *const lds = (lds_char *)lds_dyn;
+    AttentionShare my;
+    if (!my.find(p, kWavesOfAttention * 16 * RT)) return;
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    Wave w(p);
+    w.b = my.b;
+    w.g = my.g;
+    w.R = my.R;
+    w.row0 = my.group0 + wave * 16 * RT;
+    const Cache8 &c = p.cache;
+    const uint32_t nb = c.capacity >> c.block_log2;
+    const uint8_t *const keys = c.k_codes + (uint64_t)my.bg * c.capacity * c.dim, *const values = c.v_codes + (uint64_t)my.bg * c.capacity * c.vdim;
+    const float *const k_scale = c.k_scale + (uint64_t)my.bg * nb, *const v_scale = c.v_scale + (uint64_t)my.bg * nb;
+    float ks_next = 0.0f, vs_next = 0.0f;
+    auto ask = [&](uint32_t t, uint32_t place) {
+#pragma unroll
+        for (int i = 0; i < kMine; i++) { // the first two waves ask for keys, the others for values
+            const int n = wave * kMine + i;
+            const uint4 *const from = n < 4 * NL ? w.key_codes(keys, t, n / NL, n % NL) : w.value_codes(values, t, n - 4 * NL);
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from, (__attribute__((address_space(3))) void *)(lds + (place * kCodes + n) * 1024), 16, 0, 0);
+        }
+        ks_next = k_scale[w.block_of(t)];
+        vs_next = v_scale[w.block_of(t)];
+    };
+    ask(my.tile, 0);
+    uint32_t from = 0, to = 0; // tiles that the wave's rows see
+    if (w.row0 < my.R) {
+        w.begin_rows(my.held);
+        from = (uint32_t)max(w.any_from, 0) / kTile;
+        to = w.any_to < 0 ? 0 : (uint32_t)w.any_to / kTile + 1;
+    }
+    for (uint32_t t = my.tile; t < my.end_tile; t++) {
+        const uint32_t place = (t - my.tile) & 1;
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(0x0070); // vmcnt(0) lgkmcnt(0): this wave's part of the tile is in LDS, and it has read the one before
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        const float ks = ks_next, vs = vs_next;
+        if (t + 1 < my.end_tile) ask(t + 1, place ^ 1);
+        if (t < from || t >= to) continue;
+        const lds_char *const codes = lds + place * kCodes * 1024 + lane * 16;
+        auto piece = [&](int n) {
+            typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+            const u4 v = *reinterpret_cast<const __attribute__((address_space(3))) u4 *>(codes + n * 1024);
+            return make_uint4(v[0], v[1], v[2], v[3]);
+        };
+        w.scores(t, [&](int kt, int l) { return piece(kt * NL + l); });
+        w.weigh(ks);
+        bool clean = false;
+        w.products(vs, [&](int v) { return clean ? without_nan(piece(4 * NL + v)) : piece(4 * NL + v); }, [&] { clean = true; });
+    }
+    __builtin_amdgcn_s_waitcnt(0x0070); // no load may write LDS that another workgroup gets
+    if (w.row0 >= my.R) return;
+    w.end_tiles();
+    w.store(my.range.parts, my.split);
 }
 
 template <class T> int launch_cache_attention_of(const LaunchOn &on, const CacheAttentionPlan &p) {
     const dim3 grid(p.bgs * p.splits * p.row_blocks), block(64 * kWavesOfAttention);
     const uint32_t nl = (std::max(p.cache.dim, p.cache.vdim) + 63) / 64;
-    auto launch = [&](auto kernel) { return on("cache attention launch", kernel, grid, block, p); };
-    if (nl == 1) return p.rows_by_wave ? launch(cache_attention_kernel<T, 1, 2, true>) : p.two_tiles ? launch(cache_attention_kernel<T, 1, 2, false>) : launch(cache_attention_kernel<T, 1, 1, false>);
-    if (nl == 2) return p.rows_by_wave ? launch(cache_attention_kernel<T, 2, 2, true>) : p.two_tiles ? launch(cache_attention_kernel<T, 2, 2, false>) : launch(cache_attention_kernel<T, 2, 1, false>);
-    return p.rows_by_wave ? launch(cache_attention_kernel<T, 4, 1, true>) : launch(cache_attention_kernel<T, 4, 1, false>);
+    auto launch = [&](auto kernel, size_t lds = 0) { return on.with_lds("cache attention launch", kernel, grid, block, lds, p); };
+    const size_t lds = 2 * 8 * 1024 * (nl > 2 ? 4 : nl);
+    if (p.rows_by_wave)
+        return nl == 1 ? launch(cache_attention_rows_kernel<T, 1, 2>, lds) : nl == 2 ? launch(cache_attention_rows_kernel<T, 2, 2>, lds) : launch(cache_attention_rows_kernel<T, 4, 1>, lds);
+    if (nl == 1) return p.two_tiles ? launch(cache_attention_kernel<T, 1, 2>) : launch(cache_attention_kernel<T, 1, 1>);
+    if (nl == 2) return p.two_tiles ? launch(cache_attention_kernel<T, 2, 2>) : launch(cache_attention_kernel<T, 2, 1>);
+    return launch(cache_attention_kernel<T, 4, 1>);
 }
 template <class T> int load_cache_attention_of() {
     hipFuncAttributes a;
-    CG_HIP(hipFuncGetAttributes(&a, reinterpret_cast<const void *>(cache_attention_kernel<T, 1, 1, false>)));
+    CG_HIP(hipFuncGetAttributes(&a, reinterpret_cast<const void *>(cache_attention_kernel<T, 1, 1>)));
     return CG_OK;
 }
 #endif
