@@ -197,14 +197,19 @@ template <class T, int NL, int RT> struct AttentionWave {
         const int at = (int)(t * kTile);
         mine = at + (int)quad * 16;
         masked = at < all_from || at + (int)kTile - 1 > all_to;
+        uint4 codes[4][NL]; // (asked for one row of positions ahead)
+#pragma unroll
+        for (int l = 0; l < NL; l++) codes[0][l] = keys(0, l);
 #pragma unroll
         for (int kt = 0; kt < 4; kt++) {
             half8v a[kSteps];
 #pragma unroll
+            for (int l = 0; l < NL && kt < 3; l++) codes[kt + 1][l] = keys(kt + 1, l);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
             for (int l = 0; l < NL; l++) {
-                const uint4 codes = keys(kt, l);
-                a[2 * l] = eight_of(codes, 0);
-                a[2 * l + 1] = eight_of(codes, 1);
+                a[2 * l] = eight_of(codes[kt][l], 0);
+                a[2 * l + 1] = eight_of(codes[kt][l], 1);
             }
 #pragma unroll
             for (int rt = 0; rt < RT; rt++) {
@@ -338,12 +343,17 @@ template <class T, int NL, int RT> struct AttentionWave {
                     for (int v = 0; v < NV; v++) total[rt][v] *= by;
             }
             const float scale = passes == 1 || (int)quad == pass ? power_of_two(max(e - unit, -126)) : 0.0f;
+            constexpr int kAhead = 2;
+            uint4 codes[NV];
+#pragma unroll
+            for (int v = 0; v < kAhead; v++) codes[v] = values(v);
 #pragma unroll
             for (int v = 0; v < NV; v++) {
-                const uint4 codes = values(v);
                 half8v a[2];
+                if (v + kAhead < NV) codes[v + kAhead] = values(v + kAhead);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int st = 0; st < 2; st++) a[st] = eight_of(codes, st, scale);
+                for (int st = 0; st < 2; st++) a[st] = eight_of(codes[v], st, scale);
 #pragma unroll
                 for (int rt = 0; rt < RT; rt++) {
                     float4v s = kTotals ? total[rt][v] : float4v{0.0f, 0.0f, 0.0f, 0.0f};
@@ -523,9 +533,9 @@ template <class T, int NL, int RT> __global__ __launch_bounds__(64 * kWavesOfAtt
     float ks_next = 0.0f, vs_next = 0.0f;
     auto ask = [&](uint32_t t, uint32_t place) {
 #pragma unroll
-        for (int i = 0; i < kMine; i++) { // the first two waves ask for keys, the others for values
+        for (int i = 0; i < kMine; i++) {
             const int n = wave * kMine + i;
-            const uint4 *const from = n < 4 * NL ? w.key_codes(keys, t, n / NL, n % NL) : w.value_codes(values, t, n - 4 * NL);
+            const uint4 *const from = wave < 2 ? w.key_codes(keys, t, n / NL, n % NL) : w.value_codes(values, t, n - 4 * NL);
             __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from, (__attribute__((address_space(3))) void *)(lds + (place * kCodes + n) * 1024), 16, 0, 0);
         }
         ks_next = k_scale[w.block_of(t)];
