@@ -77,6 +77,7 @@ struct CacheAttentionPlan {
     uint32_t bgs, row_blocks, splits; // (sequence, kv head) pairs; blocks of a pair's rows; parts that the keys of a block of rows are cut into
     bool rows_by_wave, two_tiles;     // which kernel: see cache_attention_shape
     uint32_t rows;                    // of a pair, at most: tokens * rep
+    FastDiv rep_div, bgs_div, splits_div, heads_div; // heads: of keys and values
     float *parts;                     // splits > 1: [pair][split][row][vdim] and behind them [pair][split][row] {maximum, sum}
     float2 *stats;
 };
@@ -96,35 +97,28 @@ __device__ __forceinline__ float widened(float x) { return x; }
 __device__ __forceinline__ float widened(_Float16 x) { return (float)x; }
 __device__ __forceinline__ float widened(__bf16 x) { return (float)x; }
 
-// N consecutive elements; whole: they lie at a multiple of 16 bytes or of their own size, the smaller of the two.
-template <class T, int N> __device__ __forceinline__ void load_elements(const T *p, bool whole, float (&x)[N]) {
-    constexpr int kBytes = N * (int)sizeof(T) < 16 ? N * (int)sizeof(T) : 16, kEach = kBytes / (int)sizeof(T);
-    typedef T piece __attribute__((ext_vector_type(kEach)));
-    if (whole) {
-        piece v[N / kEach];
+// N consecutive elements, in 16-byte pieces where there are as many (the hardware takes them at any element's address; a call's
+// rows may lie at any).
+template <class T, int N> struct Pieces {
+    static constexpr int kBytes = N * (int)sizeof(T) < 16 ? N * (int)sizeof(T) : 16, kEach = kBytes / (int)sizeof(T), kCount = N / kEach;
+    typedef T Piece __attribute__((ext_vector_type(kEach), aligned(sizeof(T))));
+};
+template <class T, int N> __device__ __forceinline__ void load_elements(const T *p, float (&x)[N]) {
+    typedef Pieces<T, N> P;
+    typename P::Piece v[P::kCount];
 #pragma unroll
-        for (int i = 0; i < N / kEach; i++) v[i] = reinterpret_cast<const piece *>(p)[i];
+    for (int i = 0; i < P::kCount; i++) v[i] = reinterpret_cast<const typename P::Piece *>(p)[i];
 #pragma unroll
-        for (int i = 0; i < N; i++) x[i] = widened(v[i / kEach][i % kEach]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; i++) x[i] = widened(p[i]);
-    }
+    for (int i = 0; i < N; i++) x[i] = widened(v[i / P::kEach][i % P::kEach]);
 }
-template <class T, int N> __device__ __forceinline__ void store_elements(T *p, bool whole, const float (&x)[N]) {
-    constexpr int kBytes = N * (int)sizeof(T) < 16 ? N * (int)sizeof(T) : 16, kEach = kBytes / (int)sizeof(T);
-    typedef T piece __attribute__((ext_vector_type(kEach)));
-    if (whole) {
+template <class T, int N> __device__ __forceinline__ void store_elements(T *p, const float (&x)[N]) {
+    typedef Pieces<T, N> P;
 #pragma unroll
-        for (int i = 0; i < N / kEach; i++) {
-            piece v;
+    for (int i = 0; i < P::kCount; i++) {
+        typename P::Piece v;
 #pragma unroll
-            for (int j = 0; j < kEach; j++) v[j] = (T)x[i * kEach + j];
-            reinterpret_cast<piece *>(p)[i] = v;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; i++) p[i] = (T)x[i];
+        for (int j = 0; j < P::kEach; j++) v[j] = (T)x[i * P::kEach + j];
+        reinterpret_cast<typename P::Piece *>(p)[i] = v;
     }
 }
 // A block's scale's exponent (scales are powers of two; what else a caller's memory may hold counts as the power below, within the limits).

@@ -41,7 +41,7 @@ __device__ __forceinline__ int exponent_for(float size) {
 }
 __device__ __forceinline__ float largest_finite(float m, float x) { return fabsf(x) < INFINITY ? fmaxf(m, fabsf(x)) : m; }
 
-template <class T, int UNITS, bool VALUES> __device__ void append_block(const CacheAppendPlan &p, uint32_t b, uint32_t g, uint32_t nth, bool whole) {
+template <class T, int UNITS, bool VALUES> __device__ void append_block(const CacheAppendPlan &p, uint32_t b, uint32_t g, uint32_t nth) {
     __shared__ float sizes[kThreads / 64];
     const Cache8 &c = p.cache;
     const uint32_t n = 1u << c.block_log2, W = VALUES ? c.vdim : c.dim;
@@ -85,7 +85,7 @@ template <class T, int UNITS, bool VALUES> __device__ void append_block(const Ca
         } else {
             const uint32_t t = id / pieces, k = id - t * pieces;
             to[i] = reinterpret_cast<uint4 *>(codes + (uint64_t)(t0 + t) * W + k * kPiece);
-            load_elements<T, kPiece>(rows + (row0 + t0 + t) * pitch + k * kPiece, whole, x[i]);
+            load_elements<T, kPiece>(rows + (row0 + t0 + t) * pitch + k * kPiece, x[i]);
         }
     }
 #pragma unroll
@@ -139,15 +139,15 @@ template <class T, int UNITS, bool VALUES> __device__ void append_block(const Ca
     }
 }
 
-template <class T, int UNITS> __global__ __launch_bounds__(kThreads) void cache_append_kernel(CacheAppendPlan p, uint32_t touched, bool k_whole) {
+template <class T, int UNITS> __global__ __launch_bounds__(kThreads) void cache_append_kernel(CacheAppendPlan p, uint32_t touched) {
     uint32_t id = blockIdx.x;
     const uint32_t nth = id % touched;
     id /= touched;
     const bool values = id & 1;
     id >>= 1;
     const uint32_t g = id % p.cache.kv_heads, b = id / p.cache.kv_heads;
-    if (values) append_block<T, UNITS, true>(p, b, g, nth, false);
-    else append_block<T, UNITS, false>(p, b, g, nth, k_whole);
+    if (values) append_block<T, UNITS, true>(p, b, g, nth);
+    else append_block<T, UNITS, false>(p, b, g, nth);
 }
 
 } // namespace
@@ -157,12 +157,11 @@ int launch_cache_append(const LaunchOn &on, cg_dtype dtype, const CacheAppendPla
     const uint32_t touched = std::min(p.cache.capacity / n, (p.batch.tokens + n - 2) / n + 1);
     return with_element(dtype, [&](auto e) {
         typedef decltype(e) T;
-        const bool whole = reinterpret_cast<uintptr_t>(p.k) % 16 == 0 && p.k_pitch * sizeof(T) % 16 == 0; // (dim is a multiple of 16)
         const dim3 grid(touched * p.cache.kv_heads * p.batch.sequences * 2);
         // what a thread keeps in registers: two pieces for blocks of up to 8192 codes, eight for the largest
         return n * std::max(p.cache.dim, p.cache.vdim) <= 2 * kPiece * kThreads
-                   ? on("cache append launch", cache_append_kernel<T, 2>, grid, dim3(kThreads), p, touched, whole)
-                   : on("cache append launch", cache_append_kernel<T, 8>, grid, dim3(kThreads), p, touched, whole);
+                   ? on("cache append launch", cache_append_kernel<T, 2>, grid, dim3(kThreads), p, touched)
+                   : on("cache append launch", cache_append_kernel<T, 8>, grid, dim3(kThreads), p, touched);
     });
 }
 

@@ -33,7 +33,7 @@ template <class T> __global__ __launch_bounds__(256) void join_parts_kernel(Cach
     const uint32_t s = r / p.rep, head = g * p.rep + r - s * p.rep;
     T *const dst = static_cast<T *>(p.out) + ((int64_t)b * p.batch.tokens + s) * p.out_pitch + head * p.cache.vdim + vec * 4;
     const float y[4] = {total[0] * inv, total[1] * inv, total[2] * inv, total[3] * inv};
-    store_elements<T, 4>(dst, reinterpret_cast<uintptr_t>(p.out) % (4 * sizeof(T)) == 0 && p.out_pitch % 4 == 0, y);
+    store_elements<T, 4>(dst, y);
 }
 
 uint32_t rows_of_group(const CacheAttentionPlan &p) {
@@ -58,6 +58,10 @@ size_t shape_cache_attention(cg_dtype, CacheAttentionPlan *p) {
     uint64_t splits = groups < 512 ? (512 + groups - 1) / groups : 1;
     splits = std::max<uint64_t>(1, std::min<uint64_t>({splits, tiles / least, 256}));
     p->splits = (uint32_t)splits;
+    p->rep_div = make_fastdiv(p->rep);
+    p->bgs_div = make_fastdiv(p->bgs);
+    p->splits_div = make_fastdiv(p->splits);
+    p->heads_div = make_fastdiv(p->cache.kv_heads);
     return splits == 1 ? 0 : (size_t)p->bgs * splits * p->rows * (p->cache.vdim + 2) * 4;
 }
 

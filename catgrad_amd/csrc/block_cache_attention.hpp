@@ -82,9 +82,9 @@ __device__ __forceinline__ int quads_max(int x) {
     x = max(x, __shfl_xor(x, 16));
     return max(x, __shfl_xor(x, 32));
 }
-__device__ __forceinline__ float quads_sum(float x) {
-    x += __shfl_xor(x, 16);
-    return x + __shfl_xor(x, 32);
+__device__ __forceinline__ uint32_t quads_max(uint32_t x) {
+    x = max(x, (uint32_t)__shfl_xor((int)x, 16));
+    return max(x, (uint32_t)__shfl_xor((int)x, 32));
 }
 
 // What a wave knows of its rows, and does with a tile.  RT: 16-row groups; NL: 64-channel pieces of a head.
@@ -109,49 +109,55 @@ template <class T, int NL, int RT> struct AttentionWave {
     bool masked; // not all rows see all of it
 
     __device__ __forceinline__ AttentionWave(const CacheAttentionPlan &plan) : p(plan) {}
-    __device__ __forceinline__ int64_t token_of(int rt) const { return (int64_t)b * p.batch.tokens + min(row0 + rt * 16 + col, R - 1) / p.rep; }
+    __device__ __forceinline__ int64_t token_of(int rt) const { return (int64_t)b * p.batch.tokens + fastdiv(min(row0 + rt * 16 + col, R - 1), p.rep_div); }
 
     // The queries of rows row0 .. of a pair's R rows.
     __device__ __forceinline__ void begin_rows(uint64_t held) {
         const Cache8 &c = p.cache;
-        const bool whole_q = reinterpret_cast<uintptr_t>(p.q) % 16 == 0 && p.q_pitch * sizeof(T) % 16 == 0;
         all_from = 0, all_to = 0x7FFFFFFF, any_from = 0x7FFFFFFF, any_to = -1;
+        float x[RT][NL][16];
+        const T *src[RT];
 #pragma unroll
         for (int rt = 0; rt < RT; rt++) {
-            const uint32_t r = row0 + rt * 16 + col, rr = min(r, R - 1), s = rr / p.rep, head = g * p.rep + rr - s * p.rep;
-            const uint64_t at = held + s; // its position
+            const uint32_t rr = min(row0 + rt * 16 + col, R - 1), s = fastdiv(rr, p.rep_div);
+            src[rt] = static_cast<const T *>(p.q) + ((int64_t)b * p.batch.tokens + s) * p.q_pitch + (g * p.rep + rr - s * p.rep) * c.dim;
+        }
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+            for (int l = 0; l < NL; l++) load_elements<T, 16>(src[rt] + min(l * 64 + quad * 16, c.dim - 16), x[rt][l]); // (behind dim: the last channels again, below zeros)
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
+            const uint32_t r = row0 + rt * 16 + col;
+            const uint64_t at = held + fastdiv(min(r, R - 1), p.rep_div); // its position
             last[rt] = r < R ? (int)min(at, (uint64_t)c.capacity - 1) : -1;
             begin[rt] = p.window && at + 1 > p.window ? (int)min(at + 1 - p.window, (uint64_t)c.capacity) : 0;
-            const T *src = static_cast<const T *>(p.q) + token_of(rt) * p.q_pitch + head * c.dim;
-            float x[NL][16], size = 0.0f, bad = 0.0f;
-#pragma unroll
-            for (int l = 0; l < NL; l++) {
-                const uint32_t d = l * 64 + quad * 16;
-                if (d < c.dim) {
-                    load_elements<T, 16>(src + d, whole_q, x[l]);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 16; i++) x[l][i] = 0.0f;
-                }
-#pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    size = fmaxf(size, fabsf(x[l][i]));
-                    bad += x[l][i] * 0.0f;
-                }
-            }
-            size = quads_max(size);
-            bad = quads_sum(bad); // 0, or NaN where a value is not finite: then so are the row's scores
-            const int e = bad == 0.0f && size > 0.0f ? __builtin_amdgcn_frexp_expf(size) : 0;
-            row_factor[rt] = bad == 0.0f ? ldexpf(fabsf(p.scale) * 1.44269504088896341f, e - 8) : bad;
-            const float sign = p.scale < 0.0f ? -1.0f : 1.0f;
+            uint32_t largest = 0; // magnitude, by its bits
 #pragma unroll
             for (int l = 0; l < NL; l++)
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
-                    const float y = bad == 0.0f ? ldexpf(x[l][i], 8 - e) * sign : 0.0f;
+                    largest = max(largest, __float_as_uint(x[rt][l][i]) & 0x7FFFFFFFu);
+                }
+            largest = quads_max(largest);
+            const bool finite = largest < 0x7F800000u; // (else the row's scores are NaN)
+            const int e = finite && largest ? __builtin_amdgcn_frexp_expf(__uint_as_float(largest)) : 0;
+            row_factor[rt] = finite ? ldexpf(fabsf(p.scale) * 1.44269504088896341f, e - 8) : NAN;
+#pragma unroll
+            for (int l = 0; l < NL; l++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const float y = __builtin_amdgcn_ldexpf(x[rt][l][i], 8 - e);
                     const _Float16 h = (_Float16)y;
                     q[rt][0][2 * l + i / 8][i % 8] = h;
                     if (kPieces == 2) q[rt][kPieces - 1][2 * l + i / 8][i % 8] = (_Float16)(y - (float)h);
+                }
+#pragma unroll
+            for (int piece = 0; piece < kPieces; piece++)
+#pragma unroll
+                for (int st = 0; st < kSteps; st++) {
+                    if (p.scale < 0.0f) q[rt][piece][st] = -q[rt][piece][st];
+                    q[rt][piece][st] = finite && st / 2 * 64 + quad * 16 < c.dim ? q[rt][piece][st] : half8v{};
                 }
             if (last[rt] >= 0) {
                 all_from = max(all_from, begin[rt]);
@@ -177,18 +183,32 @@ template <class T, int NL, int RT> struct AttentionWave {
         any_to = __builtin_amdgcn_readfirstlane(any_to);
     }
 
-    // Where a tile's codes lie: those of position row kt, channel piece l, and of channel group v.  (Addresses stay within the cache: a tile
-    // may reach behind its capacity, where no row sees anything; behind dim the query is zero and any code of the same key will do, behind vdim
-    // nothing is made of the totals.)
-    __device__ __forceinline__ const uint4 *key_codes(const uint8_t *keys, uint32_t t, int kt, int l) const {
+    // Where a tile's codes lie, from an address that is the same for all lanes (tile t, position row kt or channel group v) and one of the lane's
+    // (behind dim the query is zero: any code of the same key will do).
+    __device__ __forceinline__ uint32_t key_lane(int l) const {
+        const uint32_t d = l * 64 + quad * 16;
+        return ((col >> 2) * 16 + (col & 3)) * p.cache.dim + (d < p.cache.dim ? d : 0);
+    }
+    __device__ __forceinline__ uint64_t key_tile(uint32_t t, int kt) const { return ((uint64_t)t * kTile + kt * 4) * p.cache.dim; }
+    __device__ __forceinline__ uint32_t value_lane() const {
+        const uint32_t n = p.cache.block_log2, at = quad * 16;
+        return (((at >> n) * p.cache.vdim + col) << n) + (at & ((1u << n) - 1));
+    }
+    __device__ __forceinline__ uint64_t value_tile(uint32_t t, int v) const { // (behind vdim: the last channels again; nothing is made of their totals)
+        const uint32_t n = p.cache.block_log2, at = t * kTile;
+        return (((uint64_t)(at >> n) * p.cache.vdim + min(v * 16u, p.cache.vdim - 16)) << n) + (at & ((1u << n) - 1));
+    }
+    // A tile that reaches behind the capacity, where no row sees anything: lanes there take the cache's last position or block.
+    __device__ __forceinline__ bool reaches_beyond(uint32_t t) const { return (t + 1) * kTile > p.cache.capacity; }
+    __device__ __forceinline__ uint64_t key_at_end(uint32_t t, int kt, int l) const {
         const uint32_t at = min(t * kTile + (col >> 2) * 16 + kt * 4 + (col & 3), p.cache.capacity - 1), d = l * 64 + quad * 16;
-        return reinterpret_cast<const uint4 *>(keys + (uint64_t)at * p.cache.dim + (d < p.cache.dim ? d : 0));
+        return (uint64_t)at * p.cache.dim + (d < p.cache.dim ? d : 0);
+    }
+    __device__ __forceinline__ uint64_t value_at_end(uint32_t t, int v) const {
+        const uint32_t n = p.cache.block_log2, at = (t * kTile + quad * 16) & ((1u << n) - 1);
+        return (((uint64_t)block_of(t) * p.cache.vdim + min(v * 16u, p.cache.vdim - 16) + col) << n) + at;
     }
     __device__ __forceinline__ uint32_t block_of(uint32_t t) const { return min((t * kTile + quad * 16) >> p.cache.block_log2, (p.cache.capacity >> p.cache.block_log2) - 1); }
-    __device__ __forceinline__ const uint4 *value_codes(const uint8_t *values, uint32_t t, int v) const {
-        const uint32_t n = p.cache.block_log2, at = (t * kTile + quad * 16) & ((1u << n) - 1);
-        return reinterpret_cast<const uint4 *>(values + (((uint64_t)block_of(t) * p.cache.vdim + min(v * 16u, p.cache.vdim - 16) + col) << n) + at);
-    }
 
     __device__ __forceinline__ bool sees(int rt, int i) const { return mine + i >= begin[rt] && mine + i <= last[rt]; } // i: of the lane's 16 positions
 
@@ -383,14 +403,13 @@ template <class T, int NL, int RT> struct AttentionWave {
             const float sum = sums[rt][0];
             if (parts == 1) {
                 const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-                const uint32_t head = g * p.rep + r % p.rep;
+                const uint32_t head = g * p.rep + r - fastdiv(r, p.rep_div) * p.rep;
                 T *const dst = static_cast<T *>(p.out) + token_of(rt) * p.out_pitch + head * c.vdim + quad * 4;
-                const bool whole = reinterpret_cast<uintptr_t>(p.out) % (4 * sizeof(T)) == 0 && p.out_pitch % 4 == 0;
 #pragma unroll
                 for (int v = 0; v < NV; v++) {
                     if (v * 16 >= (int)c.vdim) continue;
                     const float y[4] = {total[rt][v][0] * inv, total[rt][v][1] * inv, total[rt][v][2] * inv, total[rt][v][3] * inv};
-                    store_elements<T, 4>(dst + v * 16, whole, y);
+                    store_elements<T, 4>(dst + v * 16, y);
                 }
             } else {
                 const uint64_t at = ((uint64_t)(b * c.kv_heads + g) * p.splits + split) * p.rows + r;
@@ -411,17 +430,16 @@ struct AttentionShare {
     KeyRange range;
     uint32_t tile, end_tile;
     __device__ __forceinline__ bool find(const CacheAttentionPlan &p, uint32_t group) {
-        uint32_t id = blockIdx.x;
-        bg = id % p.bgs;
-        id /= p.bgs;
-        split = id % p.splits;
-        group0 = (p.row_blocks - 1 - id / p.splits) * group; // (the longest rows first)
-        b = bg / p.cache.kv_heads;
+        const uint32_t id = fastdiv(blockIdx.x, p.bgs_div), block = fastdiv(id, p.splits_div);
+        bg = blockIdx.x - id * p.bgs;
+        split = id - block * p.splits;
+        group0 = (p.row_blocks - 1 - block) * group; // (the longest rows first)
+        b = fastdiv(bg, p.heads_div);
         g = bg - b * p.cache.kv_heads;
         held = p.batch.held_by(b);
         R = p.batch.count_of(b) * p.rep;
         if (group0 >= R) return false;
-        range = key_range(p, held, group0 / p.rep, (min(group0 + group, R) - 1) / p.rep);
+        range = key_range(p, held, fastdiv(group0, p.rep_div), fastdiv(min(group0 + group, R) - 1, p.rep_div));
         if (split >= range.parts) return false;
         tile = range.first_tile + split * range.each;
         end_tile = min(tile + range.each, range.end_tile);
@@ -448,17 +466,33 @@ template <class T, int NL, int RT> __global__ __launch_bounds__(64 * kWavesOfAtt
     const float *const k_scale = c.k_scale + (uint64_t)my.bg * nb, *const v_scale = c.v_scale + (uint64_t)my.bg * nb;
     uint4 k_now[4][NL], v_now[NV];
     float ks_now = 0.0f, vs_now = 0.0f;
+    uint32_t key_lane[NL];
+#pragma unroll
+    for (int l = 0; l < NL; l++) key_lane[l] = w.key_lane(l);
+    const uint32_t value_lane = w.value_lane();
     auto ask_keys = [&](uint32_t t) {
-#pragma unroll
-        for (int kt = 0; kt < 4; kt++)
-#pragma unroll
-            for (int l = 0; l < NL; l++) k_now[kt][l] = *w.key_codes(keys, t, kt, l);
         ks_now = k_scale[w.block_of(t)];
+        if (w.reaches_beyond(t)) {
+#pragma unroll
+            for (int kt = 0; kt < 4; kt++)
+#pragma unroll
+                for (int l = 0; l < NL; l++) k_now[kt][l] = *reinterpret_cast<const uint4 *>(keys + w.key_at_end(t, kt, l));
+        } else {
+#pragma unroll
+            for (int kt = 0; kt < 4; kt++)
+#pragma unroll
+                for (int l = 0; l < NL; l++) k_now[kt][l] = *reinterpret_cast<const uint4 *>(keys + w.key_tile(t, kt) + key_lane[l]);
+        }
     };
     auto ask_values = [&](uint32_t t) {
-#pragma unroll
-        for (int v = 0; v < NV; v++) v_now[v] = *w.value_codes(values, t, v);
         vs_now = v_scale[w.block_of(t)];
+        if (w.reaches_beyond(t)) {
+#pragma unroll
+            for (int v = 0; v < NV; v++) v_now[v] = *reinterpret_cast<const uint4 *>(values + w.value_at_end(t, v));
+        } else {
+#pragma unroll
+            for (int v = 0; v < NV; v++) v_now[v] = *reinterpret_cast<const uint4 *>(values + w.value_tile(t, v) + value_lane);
+        }
     };
     uint32_t tile = my.tile + wave;
     if (tile < my.end_tile) {
@@ -531,12 +565,25 @@ template <class T, int NL, int RT> __global__ __launch_bounds__(64 * kWavesOfAtt
     const uint8_t *const keys = c.k_codes + (uint64_t)my.bg * c.capacity * c.dim, *const values = c.v_codes + (uint64_t)my.bg * c.capacity * c.vdim;
     const float *const k_scale = c.k_scale + (uint64_t)my.bg * nb, *const v_scale = c.v_scale + (uint64_t)my.bg * nb;
     float ks_next = 0.0f, vs_next = 0.0f;
-    auto ask = [&](uint32_t t, uint32_t place) {
+    uint32_t key_lane[NL];
 #pragma unroll
-        for (int i = 0; i < kMine; i++) {
-            const int n = wave * kMine + i;
-            const uint4 *const from = wave < 2 ? w.key_codes(keys, t, n / NL, n % NL) : w.value_codes(values, t, n - 4 * NL);
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from, (__attribute__((address_space(3))) void *)(lds + (place * kCodes + n) * 1024), 16, 0, 0);
+    for (int l = 0; l < NL; l++) key_lane[l] = w.key_lane(l);
+    const uint32_t value_lane = w.value_lane();
+    auto ask = [&](uint32_t t, uint32_t place) { // the first two waves ask for keys, the others for values
+        auto into = [&](int i, const uint8_t *from) {
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from,
+                                             (__attribute__((address_space(3))) void *)(lds + (place * kCodes + wave * kMine + i) * 1024), 16, 0, 0);
+        };
+        const uint32_t n = wave & 1; // (its half of them)
+        if (w.reaches_beyond(t)) {
+#pragma unroll
+            for (int i = 0; i < kMine; i++) into(i, wave < 2 ? keys + w.key_at_end(t, n * 2 + i / NL, i % NL) : values + w.value_at_end(t, n * kMine + i));
+        } else if (wave < 2) {
+#pragma unroll
+            for (int i = 0; i < kMine; i++) into(i, keys + w.key_tile(t, n * 2 + i / NL) + key_lane[i % NL]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kMine; i++) into(i, values + w.value_tile(t, n * kMine + i) + value_lane);
         }
         ks_next = k_scale[w.block_of(t)];
         vs_next = v_scale[w.block_of(t)];

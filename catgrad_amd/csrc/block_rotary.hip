@@ -17,7 +17,7 @@ namespace {
 constexpr uint32_t kThreads = 256, kUnits = 4; // units of a thread, all of them asked for at once
 constexpr uint32_t kMostPairs = 1024;          // cosines and sines of a workgroup
 
-// A unit is VEC pairs of a head, or VEC values behind the turned ones.  VEC 1: any alignment.
+// A unit is VEC pairs of a head, or VEC values behind the turned ones.  VEC 1: pairs that are no whole 16 bytes.
 template <class T, int VEC, bool INTERLEAVED> __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryPlan p) {
     __shared__ float2 turn[kMostPairs];
     const uint32_t pairs = p.rot / 2, all = p.batch.sequences * p.batch.tokens, first = blockIdx.x * p.group;
@@ -42,15 +42,15 @@ template <class T, int VEC, bool INTERLEAVED> __global__ __launch_bounds__(kThre
         to[i] = static_cast<T *>(is_q ? p.q_out : p.k_out) + token * (is_q ? p.q_out_pitch : p.k_out_pitch) + head * p.dim + d;
         if (pair && INTERLEAVED) {
             float z[2 * VEC];
-            load_elements<T, 2 * VEC>(src, VEC > 1, z);
+            load_elements<T, 2 * VEC>(src, z);
 #pragma unroll
             for (int j = 0; j < VEC; j++) {
                 x[i][j] = z[2 * j];
                 y[i][j] = z[2 * j + 1];
             }
         } else {
-            load_elements<T, VEC>(src, VEC > 1, x[i]);
-            if (pair) load_elements<T, VEC>(src + pairs, VEC > 1, y[i]);
+            load_elements<T, VEC>(src, x[i]);
+            if (pair) load_elements<T, VEC>(src + pairs, y[i]);
         }
         if (pair) at[i] = t * pairs + VEC * u;
     }
@@ -66,7 +66,7 @@ template <class T, int VEC, bool INTERLEAVED> __global__ __launch_bounds__(kThre
     for (uint32_t i = 0; i < kUnits; i++) {
         if (!to[i]) continue;
         if (at[i] == ~0u) {
-            store_elements<T, VEC>(to[i], VEC > 1, x[i]);
+            store_elements<T, VEC>(to[i], x[i]);
             continue;
         }
         float z[2 * VEC];
@@ -78,7 +78,7 @@ template <class T, int VEC, bool INTERLEAVED> __global__ __launch_bounds__(kThre
             z[INTERLEAVED ? 2 * j + 1 : VEC + j] = o;
         }
         if (INTERLEAVED) {
-            store_elements<T, 2 * VEC>(to[i], VEC > 1, z);
+            store_elements<T, 2 * VEC>(to[i], z);
         } else {
             float lo[VEC], hi[VEC];
 #pragma unroll
@@ -86,8 +86,8 @@ template <class T, int VEC, bool INTERLEAVED> __global__ __launch_bounds__(kThre
                 lo[j] = z[j];
                 hi[j] = z[VEC + j];
             }
-            store_elements<T, VEC>(to[i], VEC > 1, lo);
-            store_elements<T, VEC>(to[i] + pairs, VEC > 1, hi);
+            store_elements<T, VEC>(to[i], lo);
+            store_elements<T, VEC>(to[i] + pairs, hi);
         }
     }
 }
@@ -118,9 +118,7 @@ int launch_rotary(const LaunchOn &on, cg_dtype dtype, RotaryPlan p) {
     return with_element(dtype, [&](auto e) {
         typedef decltype(e) T;
         constexpr int kVec = 16 / (int)sizeof(T);
-        bool whole = p.rot / 2 % kVec == 0 && p.dim % kVec == 0;
-        for (const void *x : {p.q, (const void *)p.q_out, p.k, (const void *)p.k_out}) whole = whole && reinterpret_cast<uintptr_t>(x) % 16 == 0;
-        for (int64_t pitch : {p.q_pitch, p.q_out_pitch, p.k_pitch, p.k_out_pitch}) whole = whole && pitch % kVec == 0;
+        const bool whole = p.rot / 2 % kVec == 0 && p.dim % kVec == 0;
         return whole ? launch_vec<T, kVec>(on, p) : launch_vec<T, 1>(on, p);
     });
 }
