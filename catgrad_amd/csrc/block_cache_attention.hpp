@@ -550,6 +550,8 @@ template <class T, int NL, int RT> __global__ __launch_bounds__(64 * kWavesOfAtt
     typedef AttentionWave<T, NL, RT> Wave;
     typedef __attribute__((address_space(3))) char lds_char;
     constexpr int kCodes = 8 * NL, kMine = kCodes / kWavesOfAttention; // 1 KB pieces of a tile, of which each wave asks for some
+    constexpr int NV = Wave::NV;
+    constexpr bool kOwnCopy = NL <= 2; // (LDS for two workgroups on a compute unit)
     extern __shared__ float lds_dyn[];
     lds_char *const lds = (lds_char *)lds_dyn;
     AttentionShare my;
@@ -612,8 +614,28 @@ template <class T, int NL, int RT> __global__ __launch_bounds__(64 * kWavesOfAtt
         };
         w.scores(t, [&](int kt, int l) { return piece(kt * NL + l); });
         w.weigh(ks);
+        // codes without NaN go to memory of the wave's own (each lane reads what it wrote), so that what the products read is one address
+        // either way: a choice at every piece would keep them from being asked for ahead
+        const lds_char *values_at = codes + 4 * NL * 1024;
         bool clean = false;
-        w.products(vs, [&](int v) { return clean ? without_nan(piece(4 * NL + v)) : piece(4 * NL + v); }, [&] { clean = true; });
+        auto value = [&](int v) {
+            typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+            const u4 x = *reinterpret_cast<const __attribute__((address_space(3))) u4 *>(values_at + v * 1024);
+            return make_uint4(x[0], x[1], x[2], x[3]);
+        };
+        w.products(vs, [&](int v) { return !kOwnCopy && clean ? without_nan(value(v)) : value(v); },
+                   [&] {
+                       clean = true;
+                       if (!kOwnCopy) return;
+                       lds_char *const own = lds + (2 * kCodes + wave * NV) * 1024 + lane * 16;
+#pragma unroll
+                       for (int v = 0; v < NV; v++) {
+                           typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+                           const uint4 x = without_nan(value(v));
+                           *reinterpret_cast<__attribute__((address_space(3))) u4 *>(own + v * 1024) = u4{x.x, x.y, x.z, x.w};
+                       }
+                       values_at = own;
+                   });
     }
     __builtin_amdgcn_s_waitcnt(0x0070); // no load may write LDS that another workgroup gets
     if (w.row0 >= my.R) return;
@@ -625,7 +647,7 @@ template <class T> int launch_cache_attention_of(const LaunchOn &on, const Cache
     const dim3 grid(p.bgs * p.splits * p.row_blocks), block(64 * kWavesOfAttention);
     const uint32_t nl = (std::max(p.cache.dim, p.cache.vdim) + 63) / 64;
     auto launch = [&](auto kernel, size_t lds = 0) { return on.with_lds("cache attention launch", kernel, grid, block, lds, p); };
-    const size_t lds = 2 * 8 * 1024 * (nl > 2 ? 4 : nl);
+    const size_t lds = nl > 2 ? 2 * 32 * 1024 : nl * (2 * 8 + kWavesOfAttention * 4) * 1024; // two tiles, and the waves' copies
     if (p.rows_by_wave)
         return nl == 1 ? launch(cache_attention_rows_kernel<T, 1, 2>, lds) : nl == 2 ? launch(cache_attention_rows_kernel<T, 2, 2>, lds) : launch(cache_attention_rows_kernel<T, 4, 1>, lds);
     if (nl == 1) return p.two_tiles ? launch(cache_attention_kernel<T, 1, 2>) : launch(cache_attention_kernel<T, 1, 1>);
