@@ -42,7 +42,7 @@ struct Abi {
     CGH_FN(cg_binary) CGH_FN(cg_where) CGH_FN(cg_matmul) CGH_FN(cg_sum) CGH_FN(cg_max) CGH_FN(cg_argmax)
     CGH_FN(cg_topk) CGH_FN(cg_broadcast) CGH_FN(cg_reshape) CGH_FN(cg_transpose) CGH_FN(cg_slice)
     CGH_FN(cg_concat) CGH_FN(cg_index) CGH_FN(cg_profile_enable) CGH_FN(cg_profile_read)
-    CGH_FN(cg_realize) CGH_FN(cg_block_linear) CGH_FN(cg_block_pair_embedding) CGH_FN(cg_block_conv_linear) CGH_FN(cg_block_residual) CGH_FN(cg_block_token_side) CGH_FN(cg_block_attention) CGH_FN(cg_block_channel_delta)
+    CGH_FN(cg_realize) CGH_FN(cg_block_linear) CGH_FN(cg_block_pair_embedding) CGH_FN(cg_block_conv_linear) CGH_FN(cg_block_residual) CGH_FN(cg_block_token_side) CGH_FN(cg_block_attention) CGH_FN(cg_block_channel_delta) CGH_FN(cg_rotation_turns) CGH_FN(cg_block_rotary) CGH_FN(cg_block_cache_append) CGH_FN(cg_block_cache_attention)
 #undef CGH_FN
     void *handle = nullptr;
 
@@ -61,7 +61,7 @@ struct Abi {
         CGH_LOAD(cg_max) CGH_LOAD(cg_argmax) CGH_LOAD(cg_topk) CGH_LOAD(cg_broadcast) CGH_LOAD(cg_reshape)
         CGH_LOAD(cg_transpose) CGH_LOAD(cg_slice) CGH_LOAD(cg_concat) CGH_LOAD(cg_index)
         CGH_LOAD(cg_profile_enable) CGH_LOAD(cg_profile_read)
-        CGH_LOAD(cg_realize) CGH_LOAD(cg_block_linear) CGH_LOAD(cg_block_pair_embedding) CGH_LOAD(cg_block_conv_linear) CGH_LOAD(cg_block_residual) CGH_LOAD(cg_block_token_side) CGH_LOAD(cg_block_attention) CGH_LOAD(cg_block_channel_delta)
+        CGH_LOAD(cg_realize) CGH_LOAD(cg_block_linear) CGH_LOAD(cg_block_pair_embedding) CGH_LOAD(cg_block_conv_linear) CGH_LOAD(cg_block_residual) CGH_LOAD(cg_block_token_side) CGH_LOAD(cg_block_attention) CGH_LOAD(cg_block_channel_delta) CGH_LOAD(cg_rotation_turns) CGH_LOAD(cg_block_rotary) CGH_LOAD(cg_block_cache_append) CGH_LOAD(cg_block_cache_attention)
 #undef CGH_LOAD
     }
     Abi(const Abi &) = delete;
@@ -286,6 +286,20 @@ class Backend {
     }
     std::vector<Tensor> block_channel_delta(const cg_channel_delta_args &a) {
         return outs<3>([&](cg_tensor **o) { return abi_.cg_block_channel_delta(b_, &a, &o[0], &o[1], &o[2]); });
+    }
+    void check_rotation(const cg_rotation &r) { // (a backend refuses more than 512 values of a head)
+        double turns[256];
+        float magnitude = 0.0f;
+        check(abi_.cg_rotation_turns(&r, turns, &magnitude));
+    }
+    std::vector<Tensor> block_rotary(const cg_rotary_args &a) {
+        return outs<2>([&](cg_tensor **o) { return abi_.cg_block_rotary(b_, &a, &o[0], &o[1]); });
+    }
+    std::vector<Tensor> block_cache_append(const cg_cache_append_args &a) {
+        return outs<4>([&](cg_tensor **o) { return abi_.cg_block_cache_append(b_, &a, &o[0], &o[1], &o[2], &o[3]); });
+    }
+    Tensor block_cache_attention(const cg_cache_attention_args &a) {
+        return out([&](cg_tensor **o) { return abi_.cg_block_cache_attention(b_, &a, o); });
     }
     bool to_bool(const Tensor &x) {
         calls++;

@@ -223,5 +223,42 @@ inline std::vector<Tensor> channel_delta(I &i, DeltaTensors t, const DeltaOption
     });
 }
 
+// ---- rotary positions and a key / value cache in 8 bits (their section of include/catgrad_hip.h) ----
+// Heads at position, position + 1, .. turned -> {q, k}
+inline std::vector<Tensor> rotary(I &i, Tensor q, Tensor k, size_t heads, size_t kv_heads, size_t dim, size_t position, const cg_rotation &rotation) {
+    std::vector<std::pair<Shape, cg_dtype>> types = {{q.shape(), CG_F32}, {k.shape(), CG_F32}};
+    Operands o;
+    o.add(std::move(q));
+    o.add(std::move(k));
+    return issue(i, std::move(o), std::move(types), [heads, kv_heads, dim, position, rotation](Backend &be, auto &&raw) {
+        return be.block_rotary({raw(0), raw(1), heads, kv_heads, dim, position, rotation});
+    });
+}
+// k_codes [B, kv_heads, C, dim], v_codes [B, kv_heads, C / block, vdim, block], k_scale and v_scale [B, kv_heads, C / block]
+struct Cache8 {
+    Tensor k_codes, v_codes, k_scale, v_scale;
+};
+inline Cache8 cache_append(I &i, Tensor k, Tensor v, Cache8 c, size_t position) {
+    std::vector<std::pair<Shape, cg_dtype>> types = {{c.k_codes.shape(), CG_F8}, {c.v_codes.shape(), CG_F8}, {c.k_scale.shape(), CG_F32}, {c.v_scale.shape(), CG_F32}};
+    Operands o;
+    for (Tensor *t : {&k, &v, &c.k_codes, &c.v_codes, &c.k_scale, &c.v_scale}) o.add(std::move(*t));
+    std::vector<Tensor> r = issue(i, std::move(o), std::move(types), [position](Backend &be, auto &&raw) {
+        return be.block_cache_append({raw(0), raw(1), raw(2), raw(3), raw(4), raw(5), position});
+    });
+    return {std::move(r[0]), std::move(r[1]), std::move(r[2]), std::move(r[3])};
+}
+// softmax(scale * q . k) v of the tokens at position, position + 1, .., which the cache holds -> [B, S, heads * vdim]
+inline Tensor cache_attention(I &i, Tensor q, Cache8 c, size_t heads, size_t position, float scale, size_t window = 0) {
+    Shape s = q.shape();
+    s[2] = heads * c.v_codes.shape()[3];
+    Operands o;
+    for (Tensor *t : {&q, &c.k_codes, &c.v_codes, &c.k_scale, &c.v_scale}) o.add(std::move(*t));
+    return std::move(issue(i, std::move(o), {{s, CG_F32}}, [heads, position, scale, window](Backend &be, auto &&raw) {
+        std::vector<Tensor> r;
+        r.push_back(be.block_cache_attention({raw(0), raw(1), raw(2), raw(3), raw(4), heads, position, window, scale}));
+        return r;
+    })[0]);
+}
+
 } // namespace blocks
 } // namespace cgh

@@ -5,6 +5,7 @@
 #pragma once
 
 #include <chrono>
+#include <utility>
 
 #include "graph.hpp"
 
@@ -38,6 +39,8 @@ class Model {
     virtual void parameters_changed() {}
     // True when rows that nobody asked for skip the vocabulary projection.
     virtual bool selects_rows() const { return false; }
+    // True when a run writes into its state's memory: it is given the state itself, not clones of it, and a run that fails leaves none.
+    virtual bool takes_state() const { return false; }
 
     // `Interpreter::run(term, inputs)` for the model's term.  With Interpreter::schedule 0 the operations run as the
     // graph builder issues them; with 1 the pass is first recorded as a term and then evaluated in the layers of the
@@ -47,7 +50,9 @@ class Model {
         prepare();
         const size_t S = ids.shape()[1];
         Parts p;
-        if (i_.schedule == 0 || i_.recorder) p = def(std::move(ids), state.tensors, state.position, max_positions, want);
+        if (takes_state() && state.tensors.empty()) throw InterpreterError("an earlier run over this state has failed");
+        if (i_.schedule == 0 || i_.recorder)
+            p = def(std::move(ids), takes_state() ? std::exchange(state.tensors, {}) : state.tensors, state.position, max_positions, want);
         else p = run_recorded(std::move(ids), state.tensors, state.position, max_positions, want);
         state.tensors = std::move(p.state);
         state.position += S;

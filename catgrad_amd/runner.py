@@ -189,10 +189,12 @@ class Session:
         self._check(self._lib.cgm_vocab_size(self._s, C.byref(n)))
         self.vocab_size = int(n.value)
 
-    def load_pretrained(self, folder, dtype: str = "float32"):
-        """A model folder: config.json and model.safetensors (or the *.safetensors files in it)."""
+    def load_pretrained(self, folder, dtype: str = "float32", kv_cache: str | None = None):
+        """A model folder: config.json and model.safetensors (or the *.safetensors files in it).  kv_cache "f8" (Llama and Qwen3
+        checkpoints; also a key of config.json): keys and values are held as 8-bit codes."""
         with open(os.path.join(folder, "config.json")) as f:
-            self.load_config(f.read(), dtype)
+            config = json.load(f)
+        self.load_config({**config, "kv_cache": kv_cache} if kv_cache else config, dtype)
         files = sorted(f for f in os.listdir(folder) if f.endswith(".safetensors"))
         if not files:
             raise RuntimeError(f"{folder} holds no .safetensors file")
