@@ -436,7 +436,7 @@ int cg_block_cache_attention(cg_backend *b, const cg_cache_attention_args *a, cg
         p.cache.v_codes = static_cast<uint8_t *>(m[1]);
         p.cache.k_scale = static_cast<float *>(m[2]);
         p.cache.v_scale = static_cast<float *>(m[3]);
-        const size_t bytes = shape_cache_attention(CG_F32, &p);
+        const size_t bytes = shape_cache_attention(&p);
         if (int rc = check_launch(p)) return rc;
         Scratch tmp(b);
         if (bytes) {
@@ -519,7 +519,7 @@ int cg_cache_attention_workspace(const cg_cache_attention_rows *a, size_t *bytes
     if (no_tokens(a->batch)) return CG_OK;
     CacheAttentionPlan p;
     if (int rc = attention_from(*a, false, &p)) return rc;
-    const size_t n = shape_cache_attention(a->dtype, &p);
+    const size_t n = shape_cache_attention(&p);
     if (int rc = check_launch(p)) return rc;
     *bytes = n;
     return CG_OK;
@@ -532,7 +532,7 @@ int cg_cache_attention_noalloc(int device, const cg_cache_attention_rows *a, voi
     CacheAttentionPlan p;
     if (int rc = attention_from(*a, true, &p)) return rc;
     if (!a->q || !a->out) return fail(CG_ERR_ARG, "%s: null argument", what);
-    const size_t bytes = shape_cache_attention(a->dtype, &p);
+    const size_t bytes = shape_cache_attention(&p);
     if (int rc = check_launch(p)) return rc;
     if (bytes && (!a->workspace || a->workspace_bytes < bytes)) return fail(CG_ERR_ARG, "%s: needs a workspace of %zu bytes", what, bytes);
     if (bytes && !at16(a->workspace)) return fail(CG_ERR_ARG, "%s: the workspace lies at a multiple of 16 bytes", what);

@@ -75,14 +75,14 @@ struct CacheAttentionPlan {
     float scale;
     // by shape_cache_attention
     uint32_t bgs, row_blocks, splits; // (sequence, kv head) pairs; blocks of a pair's rows; parts that the keys of a block of rows are cut into
-    bool rows_by_wave, two_tiles;     // which kernel: see cache_attention_shape
+    bool rows_by_wave, two_tiles;     // which kernel: see shape_cache_attention
     uint32_t rows;                    // of a pair, at most: tokens * rep
     FastDiv rep_div, bgs_div, splits_div, heads_div, rows_div; // heads: of keys and values
     float *parts;                     // splits > 1: [pair][split][row][vdim] and behind them [pair][split][row] {maximum, sum}
     float2 *stats;
 };
 // Which kernel and cut a call takes, and the bytes of memory that it needs for the parts' results.
-size_t shape_cache_attention(cg_dtype dtype, CacheAttentionPlan *p);
+size_t shape_cache_attention(CacheAttentionPlan *p);
 int launch_cache_attention(const LaunchOn &on, cg_dtype dtype, const CacheAttentionPlan &p);
 
 // Loads the kernels of these files on the current device (none of them may be loaded first while a stream is captured).

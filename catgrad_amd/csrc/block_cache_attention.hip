@@ -111,7 +111,7 @@ uint32_t rows_of_group(const CacheAttentionPlan &p) {
 
 } // namespace
 
-size_t shape_cache_attention(cg_dtype, CacheAttentionPlan *p) {
+size_t shape_cache_attention(CacheAttentionPlan *p) {
     const uint32_t wide = std::max(p->cache.dim, p->cache.vdim);
     p->rows = p->batch.tokens * p->rep;
     p->bgs = p->batch.sequences * p->cache.kv_heads;

@@ -6,6 +6,7 @@
 // takes up to `group` tokens.  It asks for its first values, works out its tokens' cosines and sines meanwhile, once for all heads,
 // into LDS, and turns what has arrived.  The product of a position and a frequency is taken in 64 bits and reduced to a fraction of
 // a turn there (in 32 bits the angle at position 2^17 would be off by 2^-7); the fraction in 32 bits is off by 2^-25 of a turn.
+// Four prompts of 2048 tokens (200 MB in and out) 39 us, 5.2 TB/s (a large copy reaches 4.7); one token 2.5 us, a launch's latency.
 #include "block_cache.hpp"
 #include "device_utils.hpp"
 
