@@ -77,7 +77,7 @@ struct CacheAttentionPlan {
     uint32_t bgs, row_blocks, splits; // (sequence, kv head) pairs; blocks of a pair's rows; parts that the keys of a block of rows are cut into
     bool rows_by_wave, two_tiles;     // which kernel: see shape_cache_attention
     uint32_t rows;                    // of a pair, at most: tokens * rep
-    FastDiv rep_div, bgs_div, splits_div, heads_div, rows_div; // heads: of keys and values
+    FastDiv rep_div, bgs_div, splits_div, heads_div, rows_div, run_div; // heads: of keys and values; run: blocks of rows for a card's units
     float *parts;                     // splits > 1: [pair][split][row][vdim] and behind them [pair][split][row] {maximum, sum}
     float2 *stats;
 };

@@ -142,6 +142,7 @@ size_t shape_cache_attention(CacheAttentionPlan *p) {
     p->splits_div = make_fastdiv(p->splits);
     p->heads_div = make_fastdiv(p->cache.kv_heads);
     p->rows_div = make_fastdiv(p->rows);
+    p->run_div = make_fastdiv((uint32_t)std::max<uint64_t>(1, 256 / ((uint64_t)p->bgs * p->splits)));
     return p->splits == 1 ? 0 : (size_t)p->bgs * p->splits * p->rows * (p->cache.vdim + 2) * 4;
 }
 

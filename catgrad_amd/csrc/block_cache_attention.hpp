@@ -13,7 +13,9 @@
 //
 // Numbers.  E4M3 codes are exact in 16-bit floats.  A row of q is scaled by a power of two so that its largest magnitude lies
 // in [2^7, 2^8), and is one 16-bit float a value, or with 32-bit inputs the sum of two (2^-23 of the row's largest; 16-bit inputs are
-// exact but where they lie 2^22 below it).  A block's scale multiplies the scores in 32 bits.  Weights are exp2(score - m + 8) <= 2^15
+// exact but where they lie 2^22 below it).  Bfloat16 queries of more than 64 channels are two codes instead, the nearest and the nearest to what is left, together exact likewise:
+// then the instruction takes the keys' codes as they are (v_mfma_scale_f32_16x16x128_f8f6f4, at twice the rate, so that the two cost
+// what one 16-bit float does, without the widening of keys: four prompts of 2048 tokens of 16 heads of 128, 84 us against 89).  A block's scale multiplies the scores in 32 bits.  Weights are exp2(score - m + 8) <= 2^15
 // with m the running maximum, which moves only where a score is 7 or more above it (most tiles move none: then nothing is
 // rescaled), as one 16-bit float (2^-12) or two (2^-23), and so is their sum, by the same instruction from ones.
 // Totals are in units of a value block's scale, the codes' own scales being applied as they are widened: exact up to 2^-15 of the
@@ -26,6 +28,8 @@
 // see whole has its NaN codes of values taken out, and put back into the totals of the rows that do see them.
 #pragma once
 
+#include <type_traits>
+
 #include "block_cache.hpp"
 #include "device_utils.hpp"
 
@@ -34,6 +38,9 @@ namespace cg {
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef _Float16 half8v __attribute__((ext_vector_type(8)));
 typedef float float4v __attribute__((ext_vector_type(4)));
+typedef float float2v __attribute__((ext_vector_type(2)));
+typedef int int8v __attribute__((ext_vector_type(8)));
+typedef short short2v __attribute__((ext_vector_type(2)));
 
 constexpr uint32_t kTile = 64;           // positions of a wave's tile
 constexpr uint32_t kWavesOfAttention = 4;
@@ -92,12 +99,17 @@ template <class T, int NL, int RT> struct AttentionWave {
     static constexpr int kPieces = sizeof(T) == 4 ? 2 : 1, NV = 4 * NL, kSteps = 2 * NL;
     static constexpr bool kTotals = kPieces == 1; // the instruction adds to the totals itself
 
+    // Queries as codes, for the instructions that take both operands as such.
+    static constexpr bool kCodes = std::is_same<T, __bf16>::value && NL >= 2;
+    static constexpr int kQueryPieces = kCodes ? 2 : kPieces, kQuerySteps = kCodes ? NL / 2 : kSteps;
+    static constexpr int kLower = 5; // the second codes are in units of 2^-5
+
     const CacheAttentionPlan &p;
     const uint32_t lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
     uint32_t b, g, row0, R;
-    half8v q[RT][kPieces][kSteps];
+    typename std::conditional<kCodes, int8v, half8v>::type q[RT][kQueryPieces][kQuerySteps];
     float row_factor[RT];
-    int last[RT], begin[RT]; // positions begin .. last that the lane's rows see; none: last < begin
+    uint32_t begin[RT], seen_by[RT]; // the lane's rows see seen_by positions from begin on
     int all_from, all_to, any_from, any_to; // positions that all of the wave's rows see, that any does
     // Totals: sums of weight * value in units of 2^unit.  sums: of the weights, by the same instruction from ones.
     float4v total[RT][NV], sums[RT];
@@ -130,8 +142,9 @@ template <class T, int NL, int RT> struct AttentionWave {
         for (int rt = 0; rt < RT; rt++) {
             const uint32_t r = row0 + rt * 16 + col;
             const uint64_t at = held + fastdiv(min(r, R - 1), p.rep_div); // its position
-            last[rt] = r < R ? (int)min(at, (uint64_t)c.capacity - 1) : -1;
-            begin[rt] = p.window && at + 1 > p.window ? (int)min(at + 1 - p.window, (uint64_t)c.capacity) : 0;
+            const int last = r < R ? (int)min(at, (uint64_t)c.capacity - 1) : -1;
+            begin[rt] = last >= 0 && p.window && at + 1 > p.window ? (uint32_t)min(at + 1 - p.window, (uint64_t)c.capacity) : 0;
+            seen_by[rt] = (uint32_t)(last + 1) - begin[rt];
             uint32_t largest = 0; // magnitude, by its bits
 #pragma unroll
             for (int l = 0; l < NL; l++)
@@ -143,27 +156,49 @@ template <class T, int NL, int RT> struct AttentionWave {
             const bool finite = largest < 0x7F800000u; // (else the row's scores are NaN)
             const int e = finite && largest ? __builtin_amdgcn_frexp_expf(__uint_as_float(largest)) : 0;
             row_factor[rt] = finite ? ldexpf(fabsf(p.scale) * 1.44269504088896341f, e - 8) : NAN;
+            // times 2^(8 - e), the sign of the scale and, behind dim, zero (a row that is not finite: its factor makes its scores NaN)
+            const int up = 8 - e;
+            if (__any(up > 126)) { // (2^(8 - e) would be no float)
 #pragma unroll
-            for (int l = 0; l < NL; l++)
+                for (int l = 0; l < NL; l++)
 #pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const float y = __builtin_amdgcn_ldexpf(x[rt][l][i], 8 - e);
-                    const _Float16 h = (_Float16)y;
-                    q[rt][0][2 * l + i / 8][i % 8] = h;
-                    if (kPieces == 2) q[rt][kPieces - 1][2 * l + i / 8][i % 8] = (_Float16)(y - (float)h);
+                    for (int i = 0; i < 16; i++) x[rt][l][i] = __builtin_amdgcn_ldexpf(x[rt][l][i], max(up - 126, 0));
+            }
+            const float by = copysignf(power_of_two(min(up, 126)), p.scale);
+#pragma unroll
+            for (int l = 0; l < NL; l++) {
+                const float f = l * 64 + quad * 16 < c.dim ? by : 0.0f;
+                if constexpr (kCodes) {
+#pragma unroll
+                    for (int w = 0; w < 4; w++) {
+                        float y[4];
+#pragma unroll
+                        for (int i = 0; i < 4; i++) y[i] = x[rt][l][w * 4 + i] * f;
+                        int codes = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+                        codes = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], codes, true);
+                        const float2v a = __builtin_amdgcn_cvt_pk_f32_fp8(codes, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(codes, true);
+                        constexpr float unit_of_lower = 1.0f / (1 << kLower);
+                        short2v lower = {};
+                        lower = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(lower, y[0] - a[0], y[1] - a[1], unit_of_lower, false);
+                        lower = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(lower, y[2] - b[0], y[3] - b[1], unit_of_lower, true);
+                        q[rt][0][l / 2][l % 2 * 4 + w] = codes;
+                        q[rt][1][l / 2][l % 2 * 4 + w] = __builtin_bit_cast(int, lower);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        const float y = x[rt][l][i] * f;
+                        const _Float16 h = (_Float16)y;
+                        q[rt][0][2 * l + i / 8][i % 8] = h;
+                        if (kPieces == 2) q[rt][kPieces - 1][2 * l + i / 8][i % 8] = (_Float16)(y - (float)h);
+                    }
                 }
-#pragma unroll
-            for (int piece = 0; piece < kPieces; piece++)
-#pragma unroll
-                for (int st = 0; st < kSteps; st++) {
-                    if (p.scale < 0.0f) q[rt][piece][st] = -q[rt][piece][st];
-                    q[rt][piece][st] = finite && st / 2 * 64 + quad * 16 < c.dim ? q[rt][piece][st] : half8v{};
-                }
-            if (last[rt] >= 0) {
-                all_from = max(all_from, begin[rt]);
-                all_to = min(all_to, last[rt]);
-                any_from = min(any_from, begin[rt]);
-                any_to = max(any_to, last[rt]);
+            }
+            if (last >= 0) {
+                all_from = max(all_from, (int)begin[rt]);
+                all_to = min(all_to, last);
+                any_from = min(any_from, (int)begin[rt]);
+                any_to = max(any_to, last);
             }
             maximum[rt] = kNoMaximum;
             sums[rt] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
@@ -210,7 +245,7 @@ template <class T, int NL, int RT> struct AttentionWave {
     }
     __device__ __forceinline__ uint32_t block_of(uint32_t t) const { return min((t * kTile + quad * 16) >> p.cache.block_log2, (p.cache.capacity >> p.cache.block_log2) - 1); }
 
-    __device__ __forceinline__ bool sees(int rt, int i) const { return mine + i >= begin[rt] && mine + i <= last[rt]; } // i: of the lane's 16 positions
+    __device__ __forceinline__ bool sees(int rt, int i) const { return (uint32_t)mine - begin[rt] + (uint32_t)i < seen_by[rt]; } // i: of the lane's 16 positions
 
     // scores^T; keys(kt, l): the codes
     template <class K> __device__ __forceinline__ void scores(uint32_t t, K &&keys) {
@@ -222,23 +257,41 @@ template <class T, int NL, int RT> struct AttentionWave {
         for (int l = 0; l < NL; l++) codes[0][l] = keys(0, l);
 #pragma unroll
         for (int kt = 0; kt < 4; kt++) {
-            half8v a[kSteps];
 #pragma unroll
             for (int l = 0; l < NL && kt < 3; l++) codes[kt + 1][l] = keys(kt + 1, l);
             __builtin_amdgcn_sched_barrier(0);
+            if constexpr (kCodes) {
+                int8v a[kQuerySteps];
 #pragma unroll
-            for (int l = 0; l < NL; l++) {
-                a[2 * l] = eight_of(codes[kt][l], 0);
-                a[2 * l + 1] = eight_of(codes[kt][l], 1);
-            }
+                for (int l = 0; l < NL; l++)
 #pragma unroll
-            for (int rt = 0; rt < RT; rt++) {
-                float4v s = {0.0f, 0.0f, 0.0f, 0.0f};
+                    for (int w = 0; w < 4; w++) a[l / 2][l % 2 * 4 + w] = (int)word_of(codes[kt][l], w);
 #pragma unroll
-                for (int piece = kPieces - 1; piece >= 0; piece--)
+                for (int rt = 0; rt < RT; rt++) {
+                    float4v s = {0.0f, 0.0f, 0.0f, 0.0f};
+                    constexpr int one = 0x7F7F7F7F, lower = one - 0x01010101 * kLower; // scales: 2^(byte - 127)
 #pragma unroll
-                    for (int st = 0; st < kSteps; st++) s = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[st], q[rt][piece][st], s, 0, 0, 0);
-                score[rt][kt] = s;
+                    for (int piece = 1; piece >= 0; piece--)
+#pragma unroll
+                        for (int st = 0; st < kQuerySteps; st++) s = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a[st], q[rt][piece][st], s, 0, 0, 0, one, 0, piece ? lower : one);
+                    score[rt][kt] = s;
+                }
+            } else {
+                half8v a[kSteps];
+#pragma unroll
+                for (int l = 0; l < NL; l++) {
+                    a[2 * l] = eight_of(codes[kt][l], 0);
+                    a[2 * l + 1] = eight_of(codes[kt][l], 1);
+                }
+#pragma unroll
+                for (int rt = 0; rt < RT; rt++) {
+                    float4v s = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int piece = kPieces - 1; piece >= 0; piece--)
+#pragma unroll
+                        for (int st = 0; st < kSteps; st++) s = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[st], q[rt][piece][st], s, 0, 0, 0);
+                    score[rt][kt] = s;
+                }
             }
         }
     }
@@ -253,7 +306,7 @@ template <class T, int NL, int RT> struct AttentionWave {
             float m = -INFINITY;
             if (masked) {
 #pragma unroll
-                for (int i = 0; i < 16; i++) m = sees(rt, i) ? fmaxf(m, score[rt][i / 4][i % 4]) : m;
+                for (int i = 0; i < 16; i++) m = fmaxf(m, sees(rt, i) ? score[rt][i / 4][i % 4] : -INFINITY);
             } else {
 #pragma unroll
                 for (int i = 0; i < 16; i++) m = fmaxf(m, score[rt][i / 4][i % 4]);
@@ -433,7 +486,10 @@ struct AttentionShare {
         const uint32_t id = fastdiv(blockIdx.x, p.bgs_div), block = fastdiv(id, p.splits_div);
         bg = blockIdx.x - id * p.bgs;
         split = id - block * p.splits;
-        group0 = (p.row_blocks - 1 - block) * group; // (the longest rows first)
+        // The longest rows first, but every other run of as many as there are compute units the other way round: a unit takes one of each run, and what it
+        // takes of two adds up to as much as any other's.
+        const uint32_t run = fastdiv(block, p.run_div), begin = run * p.run_div.d;
+        group0 = (p.row_blocks - 1 - (run & 1 ? begin + min(begin + p.run_div.d, p.row_blocks) - 1 - block : block)) * group;
         b = fastdiv(bg, p.heads_div);
         g = bg - b * p.cache.kv_heads;
         held = p.batch.held_by(b);
