@@ -94,9 +94,12 @@ __device__ __forceinline__ uint32_t quads_max(uint32_t x) {
     return max(x, (uint32_t)__shfl_xor((int)x, 32));
 }
 
-// What a wave knows of its rows, and does with a tile.  RT: 16-row groups; NL: 64-channel pieces of a head.
-template <class T, int NL, int RT> struct AttentionWave {
-    static constexpr int kPieces = sizeof(T) == 4 ? 2 : 1, NV = 4 * NL, kSteps = 2 * NL;
+// What a wave knows of its rows, and does with a tile.  RT: 16-row groups; NL: 64-channel pieces of a head.  CUT: heads of at most 96
+// channels, whose second 64 are two pieces of 16 (in 16-bit floats one step of the products, of which the quads take eight channels each) and whose values
+// are six groups of 16, not eight (only where rows are many: few are bound by memory).  Portions of 3 x 500 tokens behind texts, f32 heads of 96 / 80: 86 us, 102 without.
+template <class T, int NL, int RT, bool CUT = false> struct AttentionWave {
+    static_assert(!CUT || NL == 2, "");
+    static constexpr int kPieces = sizeof(T) == 4 ? 2 : 1, NV = CUT ? 6 : 4 * NL, kSteps = CUT ? 3 : 2 * NL;
     static constexpr bool kTotals = kPieces == 1; // the instruction adds to the totals itself
 
     // Queries as codes, for the instructions that take both operands as such.
@@ -137,7 +140,7 @@ template <class T, int NL, int RT> struct AttentionWave {
 #pragma unroll
         for (int rt = 0; rt < RT; rt++)
 #pragma unroll
-            for (int l = 0; l < NL; l++) load_elements<T, 16>(src[rt] + min(l * 64 + quad * 16, c.dim - 16), x[rt][l]); // (behind dim: the last channels again, below zeros)
+            for (int l = 0; l < NL; l++) load_elements<T, 16>(src[rt] + min(channel(l), c.dim - 16), x[rt][l]); // (behind dim: the last channels again, below zeros)
 #pragma unroll
         for (int rt = 0; rt < RT; rt++) {
             const uint32_t r = row0 + rt * 16 + col;
@@ -167,7 +170,7 @@ template <class T, int NL, int RT> struct AttentionWave {
             const float by = copysignf(power_of_two(min(up, 126)), p.scale);
 #pragma unroll
             for (int l = 0; l < NL; l++) {
-                const float f = l * 64 + quad * 16 < c.dim ? by : 0.0f;
+                const float f = channel(l) < c.dim ? by : 0.0f;
                 if constexpr (kCodes) {
 #pragma unroll
                     for (int w = 0; w < 4; w++) {
@@ -186,8 +189,8 @@ template <class T, int NL, int RT> struct AttentionWave {
                     }
                 } else {
 #pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        const float y = x[rt][l][i] * f;
+                    for (int i = 0; i < (CUT && l == 1 ? 8 : 16); i++) {
+                        const float y = (CUT && l == 1 && quad >= 2 ? x[rt][l][(8 + i) % 16] : x[rt][l][i]) * f;
                         const _Float16 h = (_Float16)y;
                         q[rt][0][2 * l + i / 8][i % 8] = h;
                         if (kPieces == 2) q[rt][kPieces - 1][2 * l + i / 8][i % 8] = (_Float16)(y - (float)h);
@@ -218,10 +221,12 @@ template <class T, int NL, int RT> struct AttentionWave {
         any_to = __builtin_amdgcn_readfirstlane(any_to);
     }
 
+    // The first of the lane's 16 channels of a piece.
+    __device__ __forceinline__ uint32_t channel(int l) const { return l * 64 + (CUT && l == 1 ? quad & 1 : quad) * 16; }
     // Where a tile's codes lie, from an address that is the same for all lanes (tile t, position row kt or channel group v) and one of the lane's
     // (behind dim the query is zero: any code of the same key will do).
     __device__ __forceinline__ uint32_t key_lane(int l) const {
-        const uint32_t d = l * 64 + quad * 16;
+        const uint32_t d = channel(l);
         return ((col >> 2) * 16 + (col & 3)) * p.cache.dim + (d < p.cache.dim ? d : 0);
     }
     __device__ __forceinline__ uint64_t key_tile(uint32_t t, int kt) const { return ((uint64_t)t * kTile + kt * 4) * p.cache.dim; }
@@ -236,7 +241,7 @@ template <class T, int NL, int RT> struct AttentionWave {
     // A tile that reaches behind the capacity, where no row sees anything: lanes there take the cache's last position or block.
     __device__ __forceinline__ bool reaches_beyond(uint32_t t) const { return (t + 1) * kTile > p.cache.capacity; }
     __device__ __forceinline__ uint64_t key_at_end(uint32_t t, int kt, int l) const {
-        const uint32_t at = min(t * kTile + (col >> 2) * 16 + kt * 4 + (col & 3), p.cache.capacity - 1), d = l * 64 + quad * 16;
+        const uint32_t at = min(t * kTile + (col >> 2) * 16 + kt * 4 + (col & 3), p.cache.capacity - 1), d = channel(l);
         return (uint64_t)at * p.cache.dim + (d < p.cache.dim ? d : 0);
     }
     __device__ __forceinline__ uint64_t value_at_end(uint32_t t, int v) const {
@@ -280,8 +285,13 @@ template <class T, int NL, int RT> struct AttentionWave {
                 half8v a[kSteps];
 #pragma unroll
                 for (int l = 0; l < NL; l++) {
-                    a[2 * l] = eight_of(codes[kt][l], 0);
-                    a[2 * l + 1] = eight_of(codes[kt][l], 1);
+                    const uint4 &k = codes[kt][l];
+                    if (CUT && l == 1) {
+                        a[2] = eight_of(quad < 2 ? k.x : k.z, quad < 2 ? k.y : k.w, 1.0f);
+                        continue;
+                    }
+                    a[2 * l] = eight_of(k, 0);
+                    a[2 * l + 1] = eight_of(k, 1);
                 }
 #pragma unroll
                 for (int rt = 0; rt < RT; rt++) {
@@ -602,11 +612,11 @@ template <class T, int NL, int RT> __global__ __launch_bounds__(64 * kWavesOfAtt
 
 // Many rows: every wave of a workgroup has rows of its own, and all walk the same tiles, whose codes come straight into LDS, a tile ahead, in
 // the order in which the lanes take them.  Bound by the vector instructions between the products (widening codes, weights).
-template <class T, int NL, int RT> __global__ __launch_bounds__(64 * kWavesOfAttention, 2) void cache_attention_rows_kernel(CacheAttentionPlan p) {
-    typedef AttentionWave<T, NL, RT> Wave;
+template <class T, int NL, int RT, bool CUT = false> __global__ __launch_bounds__(64 * kWavesOfAttention, 2) void cache_attention_rows_kernel(CacheAttentionPlan p) {
+    typedef AttentionWave<T, NL, RT, CUT> Wave;
     typedef __attribute__((address_space(3))) char lds_char;
-    constexpr int kCodes = 8 * NL, kMine = kCodes / kWavesOfAttention; // 1 KB pieces of a tile, of which each wave asks for some
     constexpr int NV = Wave::NV;
+    constexpr int kKeys = 4 * NL, kCodes = kKeys + NV; // 1 KB pieces of a tile, of which each wave asks for some
     constexpr bool kOwnCopy = NL <= 2; // (LDS for two workgroups on a compute unit)
     extern __shared__ float lds_dyn[];
     lds_char *const lds = (lds_char *)lds_dyn;
@@ -628,20 +638,26 @@ template <class T, int NL, int RT> __global__ __launch_bounds__(64 * kWavesOfAtt
     for (int l = 0; l < NL; l++) key_lane[l] = w.key_lane(l);
     const uint32_t value_lane = w.value_lane();
     auto ask = [&](uint32_t t, uint32_t place) { // the first two waves ask for keys, the others for values
-        auto into = [&](int i, const uint8_t *from) {
+        auto into = [&](uint32_t i, const uint8_t *from) {
             __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from,
-                                             (__attribute__((address_space(3))) void *)(lds + (place * kCodes + wave * kMine + i) * 1024), 16, 0, 0);
+                                             (__attribute__((address_space(3))) void *)(lds + (place * kCodes + i) * 1024), 16, 0, 0);
         };
         const uint32_t n = wave & 1; // (its half of them)
+        constexpr int kHalfKeys = kKeys / 2, kHalfValues = NV / 2;
+        const uint32_t k0 = n * kHalfKeys, v0 = n * kHalfValues;
         if (w.reaches_beyond(t)) {
 #pragma unroll
-            for (int i = 0; i < kMine; i++) into(i, wave < 2 ? keys + w.key_at_end(t, n * 2 + i / NL, i % NL) : values + w.value_at_end(t, n * kMine + i));
+            for (int i = 0; i < kHalfKeys; i++)
+                if (wave < 2) into(k0 + i, keys + w.key_at_end(t, n * 2 + i / NL, i % NL));
+#pragma unroll
+            for (int i = 0; i < kHalfValues; i++)
+                if (wave >= 2) into(kKeys + v0 + i, values + w.value_at_end(t, v0 + i));
         } else if (wave < 2) {
 #pragma unroll
-            for (int i = 0; i < kMine; i++) into(i, keys + w.key_tile(t, n * 2 + i / NL) + key_lane[i % NL]);
+            for (int i = 0; i < kHalfKeys; i++) into(k0 + i, keys + w.key_tile(t, n * 2 + i / NL) + key_lane[i % NL]);
         } else {
 #pragma unroll
-            for (int i = 0; i < kMine; i++) into(i, values + w.value_tile(t, n * kMine + i) + value_lane);
+            for (int i = 0; i < kHalfValues; i++) into(kKeys + v0 + i, values + w.value_tile(t, v0 + i) + value_lane);
         }
         ks_next = k_scale[w.block_of(t)];
         vs_next = v_scale[w.block_of(t)];
@@ -672,7 +688,7 @@ template <class T, int NL, int RT> __global__ __launch_bounds__(64 * kWavesOfAtt
         w.weigh(ks);
         // codes without NaN go to memory of the wave's own (each lane reads what it wrote), so that what the products read is one address
         // either way: a choice at every piece would keep them from being asked for ahead
-        const lds_char *values_at = codes + 4 * NL * 1024;
+        const lds_char *values_at = codes + kKeys * 1024;
         bool clean = false;
         auto value = [&](int v) {
             typedef uint32_t u4 __attribute__((ext_vector_type(4)));
@@ -703,9 +719,11 @@ template <class T> int launch_cache_attention_of(const LaunchOn &on, const Cache
     const dim3 grid(p.bgs * p.splits * p.row_blocks), block(64 * kWavesOfAttention);
     const uint32_t nl = (std::max(p.cache.dim, p.cache.vdim) + 63) / 64;
     auto launch = [&](auto kernel, size_t lds = 0) { return on.with_lds("cache attention launch", kernel, grid, block, lds, p); };
-    const size_t lds = nl > 2 ? 2 * 32 * 1024 : nl * (2 * 8 + kWavesOfAttention * 4) * 1024; // two tiles, and the waves' copies
-    if (p.rows_by_wave)
-        return nl == 1 ? launch(cache_attention_rows_kernel<T, 1, 2>, lds) : nl == 2 ? launch(cache_attention_rows_kernel<T, 2, 2>, lds) : launch(cache_attention_rows_kernel<T, 4, 1>, lds);
+    if (p.rows_by_wave) { // LDS: two tiles, and the waves' copies
+        if (nl == 1) return launch(cache_attention_rows_kernel<T, 1, 2>, (2 * 8 + kWavesOfAttention * 4) * 1024);
+        if (nl == 2 && std::max(p.cache.dim, p.cache.vdim) <= 96) return launch(cache_attention_rows_kernel<T, 2, 2, true>, (2 * 14 + kWavesOfAttention * 6) * 1024);
+        return nl == 2 ? launch(cache_attention_rows_kernel<T, 2, 2>, (2 * 16 + kWavesOfAttention * 8) * 1024) : launch(cache_attention_rows_kernel<T, 4, 1>, 2 * 32 * 1024);
+    }
     if (nl == 1) return p.two_tiles ? launch(cache_attention_kernel<T, 1, 2>) : launch(cache_attention_kernel<T, 1, 1>);
     if (nl == 2) return p.two_tiles ? launch(cache_attention_kernel<T, 2, 2>) : launch(cache_attention_kernel<T, 2, 1>);
     return launch(cache_attention_kernel<T, 4, 1>);
