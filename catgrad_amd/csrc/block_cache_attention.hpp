@@ -13,8 +13,8 @@
 //
 // Numbers.  E4M3 codes are exact in 16-bit floats.  A row of q is scaled by a power of two so that its largest magnitude lies
 // in [2^7, 2^8), and is one 16-bit float a value, or with 32-bit inputs the sum of two (2^-23 of the row's largest; 16-bit inputs are
-// exact but where they lie 2^22 below it).  Bfloat16 queries of more than 64 channels are two codes instead, the nearest and the nearest to what is left, together exact likewise:
-// then the instruction takes the keys' codes as they are (v_mfma_scale_f32_16x16x128_f8f6f4, at twice the rate, so that the two cost
+// exact but where they lie 2^22 below it).  Bfloat16 queries of more than 64 channels are two codes instead, the nearest and the nearest to what is left, together exact but
+// where they lie 2^14 below the row's largest (there to 2^-22 of it): then the instruction takes the keys' codes as they are (v_mfma_scale_f32_16x16x128_f8f6f4, at twice the rate, so that the two cost
 // what one 16-bit float does, without the widening of keys: four prompts of 2048 tokens of 16 heads of 128, 84 us against 89).  A block's scale multiplies the scores in 32 bits.  Weights are exp2(score - m + 8) <= 2^15
 // with m the running maximum, which moves only where a score is 7 or more above it (most tiles move none: then nothing is
 // rescaled), as one 16-bit float (2^-12) or two (2^-23), and so is their sum, by the same instruction from ones.
@@ -105,6 +105,7 @@ template <class T, int NL, int RT, bool CUT = false> struct AttentionWave {
     // Queries as codes, for the instructions that take both operands as such.
     static constexpr bool kCodes = std::is_same<T, __bf16>::value && NL >= 2;
     static constexpr int kQueryPieces = kCodes ? 2 : kPieces, kQuerySteps = kCodes ? NL / 2 : kSteps;
+    static constexpr bool kHalves = CUT && !kCodes; // quads 2 and 3 take the second eight channels of what 0 and 1 take
     static constexpr int kLower = 5; // the second codes are in units of 2^-5
 
     const CacheAttentionPlan &p;
@@ -189,8 +190,8 @@ template <class T, int NL, int RT, bool CUT = false> struct AttentionWave {
                     }
                 } else {
 #pragma unroll
-                    for (int i = 0; i < (CUT && l == 1 ? 8 : 16); i++) {
-                        const float y = (CUT && l == 1 && quad >= 2 ? x[rt][l][(8 + i) % 16] : x[rt][l][i]) * f;
+                    for (int i = 0; i < (kHalves && l == 1 ? 8 : 16); i++) {
+                        const float y = (kHalves && l == 1 && quad >= 2 ? x[rt][l][(8 + i) % 16] : x[rt][l][i]) * f;
                         const _Float16 h = (_Float16)y;
                         q[rt][0][2 * l + i / 8][i % 8] = h;
                         if (kPieces == 2) q[rt][kPieces - 1][2 * l + i / 8][i % 8] = (_Float16)(y - (float)h);
@@ -222,7 +223,7 @@ template <class T, int NL, int RT, bool CUT = false> struct AttentionWave {
     }
 
     // The first of the lane's 16 channels of a piece.
-    __device__ __forceinline__ uint32_t channel(int l) const { return l * 64 + (CUT && l == 1 ? quad & 1 : quad) * 16; }
+    __device__ __forceinline__ uint32_t channel(int l) const { return l * 64 + (kHalves && l == 1 ? quad & 1 : quad) * 16; }
     // Where a tile's codes lie, from an address that is the same for all lanes (tile t, position row kt or channel group v) and one of the lane's
     // (behind dim the query is zero: any code of the same key will do).
     __device__ __forceinline__ uint32_t key_lane(int l) const {
@@ -286,7 +287,7 @@ template <class T, int NL, int RT, bool CUT = false> struct AttentionWave {
 #pragma unroll
                 for (int l = 0; l < NL; l++) {
                     const uint4 &k = codes[kt][l];
-                    if (CUT && l == 1) {
+                    if (kHalves && l == 1) {
                         a[2] = eight_of(quad < 2 ? k.x : k.z, quad < 2 ? k.y : k.w, 1.0f);
                         continue;
                     }

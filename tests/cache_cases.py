@@ -5,7 +5,8 @@ Tolerances.  A rounding is off by at most half a step, HALF[dtype] relative to t
 2^-25 of a turn (2^-22.3 as an angle), cosine and sine two steps of 2^-24 each, three more roundings: below 2^-20 of the pair's size
 together.  Attention: a score is off by 2^-23 of its row's largest query value times the key's values added up (the query's
 pieces), as much again for the rounding of the products' sums, 2^-22 for its exponent: in all TERMS = 2^-21 of `terms` and
-2^-20; a weight is off by that and by its own rounding (2^-22 in two pieces, 2^-11 in one), in the numerator and in the sum."""
+2^-20 (bfloat16 queries may be two codes of four bits, the second in steps of 2^-14 where the row's largest is 2^7 or more: off by
+half of one, 2^-22 of the largest, so 2^-22 + 2^-23 + 2^-22 < 2^-20 of `terms`); a weight is off by that and by its own rounding (2^-22 in two pieces, 2^-11 in one), in the numerator and in the sum."""
 import ctypes as C
 
 import numpy as np
@@ -17,6 +18,7 @@ from catgrad_amd import F16, F32, BF16, _abi as A
 TYPES = {"f32": (torch.float32, F32), "f16": (torch.float16, F16), "bf16": (torch.bfloat16, BF16)}
 HALF = {"f32": 2.0 ** -24, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}
 WEIGHT = {"f32": 2.0 ** -22, "f16": 2.0 ** -11, "bf16": 2.0 ** -11}
+TERMS = {"f32": 2.0 ** -21, "f16": 2.0 ** -21, "bf16": 2.0 ** -20}
 TINY = {"f32": 2.0 ** -149, "f16": 2.0 ** -25, "bf16": 2.0 ** -134}  # half a step of the smallest values
 
 
@@ -285,7 +287,7 @@ def run_attend(lib, device, cache, dtype, held, counts, q, H, window=0, scale=No
                 k, v = cache.heads[b][g][0].x, cache.heads[b][g][1].x
                 mine = slice(g * rep, (g + 1) * rep)
                 want, size, terms = R.attend(x[b, s, mine], held[b] + s, k, v, scale, window)
-                tol = (2 * (2.0 ** -21 * terms + 2.0 ** -20 + WEIGHT[dtype])) * size + HALF[dtype] * np.abs(want) + TINY[dtype]
+                tol = (2 * (TERMS[dtype] * terms + 2.0 ** -20 + WEIGHT[dtype])) * size + HALF[dtype] * np.abs(want) + TINY[dtype]
                 off_by(y[b, s, mine], want, tol, f"attention {what} sequence {b} token {s} head {g}")
     assert out.untouched(real), "attention wrote what is not its own"
     return out
@@ -326,8 +328,8 @@ ATTEND = {  # dtype, heads, kv heads, dim, vdim, capacity, block, held, counts, 
 }
 
 
-def run_attend_case(lib, device, name, seed=0):
-    dtype, H, G, D, V, capacity, block, held, counts, S, window, wide, skew = ATTEND[name]
+def run_attend_case(lib, device, name, seed=0, cases=ATTEND):
+    dtype, H, G, D, V, capacity, block, held, counts, S, window, wide, skew = cases[name]
     rng = np.random.default_rng(seed + len(name))
     B = len(held)
     for stale in (0xFF, 0x7E):
