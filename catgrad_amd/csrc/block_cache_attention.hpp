@@ -127,11 +127,10 @@ template <class T, int NL, int RT, bool CUT = false> struct AttentionWave {
     __device__ __forceinline__ AttentionWave(const CacheAttentionPlan &plan) : p(plan) {}
     __device__ __forceinline__ int64_t token_of(int rt) const { return (int64_t)b * p.batch.tokens + fastdiv(min(row0 + rt * 16 + col, R - 1), p.rep_div); }
 
-    // The queries of rows row0 .. of a pair's R rows.
-    __device__ __forceinline__ void begin_rows(uint64_t held) {
+    // The queries of rows row0 .. of a pair's R rows: asked for, and made ready.
+    typedef float Queries[RT][NL][16];
+    __device__ __forceinline__ void ask_rows(Queries &x) const {
         const Cache8 &c = p.cache;
-        all_from = 0, all_to = 0x7FFFFFFF, any_from = 0x7FFFFFFF, any_to = -1;
-        float x[RT][NL][16];
         const T *src[RT];
 #pragma unroll
         for (int rt = 0; rt < RT; rt++) {
@@ -142,6 +141,10 @@ template <class T, int NL, int RT, bool CUT = false> struct AttentionWave {
         for (int rt = 0; rt < RT; rt++)
 #pragma unroll
             for (int l = 0; l < NL; l++) load_elements<T, 16>(src[rt] + min(channel(l), c.dim - 16), x[rt][l]); // (behind dim: the last channels again, below zeros)
+    }
+    __device__ __forceinline__ void begin_rows(Queries &x, uint64_t held) {
+        const Cache8 &c = p.cache;
+        all_from = 0, all_to = 0x7FFFFFFF, any_from = 0x7FFFFFFF, any_to = -1;
 #pragma unroll
         for (int rt = 0; rt < RT; rt++) {
             const uint32_t r = row0 + rt * 16 + col;
@@ -566,7 +569,9 @@ template <class T, int NL, int RT> __global__ __launch_bounds__(64 * kWavesOfAtt
         ask_keys(tile);
         ask_values(tile);
     }
-    w.begin_rows(my.held);
+    typename Wave::Queries x;
+    w.ask_rows(x);
+    w.begin_rows(x, my.held);
     for (; tile < my.end_tile; tile += kWavesOfAttention) {
         const bool more = tile + kWavesOfAttention < my.end_tile;
         w.scores(tile, [&](int kt, int l) { return k_now[kt][l]; });
@@ -663,10 +668,12 @@ template <class T, int NL, int RT, bool CUT = false> __global__ __launch_bounds_
         ks_next = k_scale[w.block_of(t)];
         vs_next = v_scale[w.block_of(t)];
     };
-    ask(my.tile, 0);
     uint32_t from = 0, to = 0; // tiles that the wave's rows see
+    typename Wave::Queries x;
+    if (w.row0 < my.R) w.ask_rows(x); // (in front of the tile: they are wanted first)
+    ask(my.tile, 0);
     if (w.row0 < my.R) {
-        w.begin_rows(my.held);
+        w.begin_rows(x, my.held);
         from = (uint32_t)max(w.any_from, 0) / kTile;
         to = w.any_to < 0 ? 0 : (uint32_t)w.any_to / kTile + 1;
     }
