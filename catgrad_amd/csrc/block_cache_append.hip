@@ -143,17 +143,17 @@ template <class T, int UNITS, bool VALUES> __device__ void append_block(const Ca
 
 // One token a sequence, as in every step of a decoder: a wave takes a head's keys or values, a lane four channels of them.  Nothing of
 // the block is read but its scale, unless that grows: then every lane rounds anew what lies in its own channels' (values) or
-// places' (keys) bytes, and no lane touches another's.  64 sequences of 8 heads
-// of 128 bf16 channels, each on lines of its own in a cache that no L2 holds: 4.3 us, all of it latency (a launch, the positions held, the scale), where
-// the workgroups below take 6.4; from two tokens on those are no slower.
+// places' (keys) bytes, and no lane touches another's.  64 sequences of 8 heads of 128 bf16
+// channels: 4.3 us, all of it latency (a launch, the positions held, the scale and the token), where the workgroups above take 6.4 for their barrier, their
+// four times as many waves and the pieces of the block that a value is put into.
 template <class T, bool VALUES> __device__ void append_token(const CacheAppendPlan &p, uint32_t b, uint32_t g, uint32_t lane) {
     const Cache8 &c = p.cache;
     const uint32_t n = 1u << c.block_log2, W = VALUES ? c.vdim : c.dim, d = lane * 4;
     const bool mine = d < W;
-    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (mine) load_elements<T, 4>(static_cast<const T *>(VALUES ? p.v : p.k) + (int64_t)b * (VALUES ? p.v_pitch : p.k_pitch) + g * W + d, x);
     const uint64_t held = p.batch.held_by(b), j = held >> c.block_log2;
     if (held >= c.capacity || !p.batch.count_of(b)) return;
+    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (mine) load_elements<T, 4>(static_cast<const T *>(VALUES ? p.v : p.k) + (int64_t)b * (VALUES ? p.v_pitch : p.k_pitch) + g * W + d, x);
     const uint32_t t = (uint32_t)held & (n - 1);
     const uint64_t bg = (uint64_t)b * c.kv_heads + g, nb = c.capacity >> c.block_log2;
     float *const scale = (VALUES ? c.v_scale : c.k_scale) + bg * nb + j;
