@@ -518,7 +518,8 @@ struct AttentionShare {
 };
 
 // Few rows: the waves of a workgroup have the same rows, take their tiles in turns, codes straight to registers, and add their results up
-// in LDS.  Bound by memory.
+// in LDS.  Bound by memory: a token each of 32 sequences behind 16300 (bf16, 32 heads of 128 on 8, 1.07 GB) 160 us, 6.7 TB/s; one behind 131000
+// (f32, 268 MB) 51 us, 5.2 TB/s.
 template <class T, int NL, int RT> __global__ __launch_bounds__(64 * kWavesOfAttention, NL * RT > 2 ? 1 : 2) void cache_attention_kernel(CacheAttentionPlan p) {
     typedef AttentionWave<T, NL, RT> Wave;
     constexpr int NV = Wave::NV;
@@ -617,7 +618,9 @@ template <class T, int NL, int RT> __global__ __launch_bounds__(64 * kWavesOfAtt
 }
 
 // Many rows: every wave of a workgroup has rows of its own, and all walk the same tiles, whose codes come straight into LDS, a tile ahead, in
-// the order in which the lanes take them.  Bound by the vector instructions between the products (widening codes, weights).
+// the order in which the lanes take them.  Bound by the vector instructions between the products (widening codes, weights): four prompts of 2048 tokens (bf16,
+// 16 heads of 128 on 8, 69 GFLOP) 83 us in a run of calls, matrix pipes busy for 29 % of the cycles, vector instructions for 43 %; of the 31 us of a workgroup of 9 to 16
+// tiles 6 to 8 are its beginning and end.  128 rows share what a tile costs to fetch; with 16 a wave the widening would be done twice as often.
 template <class T, int NL, int RT, bool CUT = false> __global__ __launch_bounds__(64 * kWavesOfAttention, 2) void cache_attention_rows_kernel(CacheAttentionPlan p) {
     typedef AttentionWave<T, NL, RT, CUT> Wave;
     typedef __attribute__((address_space(3))) char lds_char;
