@@ -120,3 +120,25 @@ def test_load_pretrained(session, tmp_path):
     np.testing.assert_array_equal(session.step(1, [1, 2, 3], rows=[2]), got[1])
     session.end(1)
     assert not np.array_equal(got[0], got[1])
+
+
+@pytest.mark.parametrize("scaling", [None, {}, {"rope_type": "default"}, {"type": "linear", "factor": 1.0}], ids=str)
+def test_scaling_that_scales_nothing(session, scaling):
+    params = params_of(TINY_LLAMA, seed=3, scale=4.0)
+    got = []
+    for more in ({}, {"rope_scaling": scaling}):
+        cases.load(session, TINY_LLAMA, params, **more)
+        got.append(session.step(1, range(20), rows=range(20)))
+        session.end(1)
+    np.testing.assert_array_equal(got[0], got[1])
+
+
+def test_a_batch_is_its_sequences(session):
+    """Logits of whole prompts side by side, through `forward`, are those of each alone."""
+    params = params_of(TINY_LLAMA, seed=3, scale=4.0)
+    cases.load(session, TINY_LLAMA, params)
+    prompt = np.stack(cases.tokens_of(TINY_LLAMA, (70, 70, 70), 4))
+    _, logits = session.forward(prompt)
+    for b in range(3):
+        np.testing.assert_array_equal(session.step(b, prompt[b], rows=range(70)), logits[b])
+        session.end(b)
