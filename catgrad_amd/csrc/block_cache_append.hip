@@ -80,9 +80,10 @@ template <class T, int UNITS, bool VALUES> __device__ void append_block(const Ca
             to[i] = reinterpret_cast<uint4 *>(codes + (uint64_t)d * n + piece[i]);
             old[i] = *to[i];
 #pragma unroll
-            for (uint32_t q = 0; q < kPiece; q++) {
+            for (uint32_t q = 0; q < kPiece; q++) { // (places that are not new: a new one's value, then zero, so that no load hangs on a branch)
                 const uint32_t t = piece[i] + q;
-                x[i][q] = t >= t0 && t < t1 ? widened(rows[(row0 + t) * pitch + d]) : 0.0f;
+                const float v = widened(rows[(row0 + min(max(t, t0), t1 - 1)) * pitch + d]);
+                x[i][q] = t >= t0 && t < t1 ? v : 0.0f;
             }
         } else {
             const uint32_t t = id / pieces, k = id - t * pieces;
