@@ -71,7 +71,7 @@ template <class T, int UNITS, bool VALUES> __device__ void append_block(const Ca
     float size = 0.0f;
 #pragma unroll
     for (int i = 0; i < UNITS; i++) {
-        const uint32_t id = i * kThreads + threadIdx.x;
+        const uint32_t id = i * blockDim.x + threadIdx.x;
         to[i] = nullptr;
         if (id >= units) continue;
         if (VALUES) {
@@ -100,7 +100,8 @@ template <class T, int UNITS, bool VALUES> __device__ void append_block(const Ca
     for (int o = 32; o > 0; o >>= 1) size = fmaxf(size, __shfl_xor(size, o));
     if (threadIdx.x % 64 == 0) sizes[threadIdx.x / 64] = size;
     __syncthreads();
-    size = fmaxf(fmaxf(sizes[0], sizes[1]), fmaxf(sizes[2], sizes[3]));
+    size = sizes[0];
+    for (uint32_t i = 1; i < blockDim.x / 64; i++) size = fmaxf(size, sizes[i]);
     const int e = max(had, exponent_for(size)); // (a size of 0: the lowest)
     const bool grew = t0 && e > had;
     const float inv = power_of_two(-e), down = power_of_two(max(had - e, -64)); // (2^-64 leaves nothing of any code)
@@ -130,7 +131,7 @@ template <class T, int UNITS, bool VALUES> __device__ void append_block(const Ca
     if (!grew) return;
     // pieces that hold older positions alone
     const uint32_t rest = VALUES ? t0 / kPiece * W : t0 * pieces;
-    for (uint32_t id = threadIdx.x; id < rest; id += kThreads) {
+    for (uint32_t id = threadIdx.x; id < rest; id += blockDim.x) {
         uint4 *at;
         if (VALUES) {
             const uint32_t k = id / W, d = id - k * W;
@@ -224,10 +225,10 @@ int launch_cache_append(const LaunchOn &on, cg_dtype dtype, const CacheAppendPla
         typedef decltype(e) T;
         if (p.batch.tokens == 1) return on("cache append launch", cache_append_token_kernel<T>, dim3(p.batch.sequences * p.cache.kv_heads * 2), dim3(64), p);
         const dim3 grid(touched * p.cache.kv_heads * p.batch.sequences * 2);
-        // what a thread keeps in registers: two pieces for blocks of up to 8192 codes, eight for the largest
-        return n * std::max(p.cache.dim, p.cache.vdim) <= 2 * kPiece * kThreads
-                   ? on("cache append launch", cache_append_kernel<T, 2>, grid, dim3(kThreads), p, touched)
-                   : on("cache append launch", cache_append_kernel<T, 8>, grid, dim3(kThreads), p, touched);
+        // a thread for a piece of a block, up to 256; what one keeps in registers: two pieces for blocks of up to 8192 codes, eight for the largest
+        const uint32_t pieces = n * std::max(p.cache.dim, p.cache.vdim) / kPiece, threads = std::min(kThreads, (pieces + 63) / 64 * 64);
+        return pieces <= 2 * kThreads ? on("cache append launch", cache_append_kernel<T, 2>, grid, dim3(threads), p, touched)
+                                      : on("cache append launch", cache_append_kernel<T, 8>, grid, dim3(threads), p, touched);
     });
 }
 
