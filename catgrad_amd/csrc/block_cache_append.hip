@@ -6,8 +6,8 @@
 // channel: a thread takes 16 neighbouring positions of a channel, reads them from 16 rows (a wave's lanes take neighbouring
 // channels) and stores them in one piece, together with what the piece held of older positions.  No two workgroups share a byte
 // that either writes.  A block that grew has the rest of its codes rounded anew in a second sweep, which few appends need.
-// Bound by memory: 4 prompts of 2048 tokens (f32, 8 heads of 64) 12.0 us, 3.5 TB/s with the launch, 10.2 when inputs lie in the shared caches;
-// short ragged ones by latency: 7 of up to 301 tokens (f16, 6 heads of 80 / 96) 8.2 us for 6.7 MB.
+// Bound by memory: 4 prompts of 2048 tokens (f32, 8 heads of 128, 84 MB) 18.4 us, 4.6 TB/s; short ragged ones by latency: 7 of up to
+// 301 tokens (f16, 6 heads of 80 / 96, 6.7 MB) 6.4 us.
 #include "block_cache.hpp"
 #include "device_utils.hpp"
 
@@ -16,7 +16,7 @@
 namespace cg {
 namespace {
 
-constexpr uint32_t kThreads = 256, kPiece = 16; // bytes (codes) of a unit of work
+constexpr uint32_t kThreads = 512, kPiece = 16; // bytes (codes) of a unit of work
 
 __device__ __forceinline__ float code_range(float x) { // within the codes' range; NaN stays
     const float c = __builtin_amdgcn_fmed3f(x, -448.0f, 448.0f);
@@ -225,16 +225,17 @@ int launch_cache_append(const LaunchOn &on, cg_dtype dtype, const CacheAppendPla
         typedef decltype(e) T;
         if (p.batch.tokens == 1) return on("cache append launch", cache_append_token_kernel<T>, dim3(p.batch.sequences * p.cache.kv_heads * 2), dim3(64), p);
         const dim3 grid(touched * p.cache.kv_heads * p.batch.sequences * 2);
-        // a thread for a piece of a block, up to 256; what one keeps in registers: two pieces for blocks of up to 8192 codes, eight for the largest
+        // a thread for a piece of a block, up to 512, then up to four of the largest blocks' pieces a thread (2 x 500 tokens, f32, heads of 256 in blocks of 128: 12.0 us;
+        // with half as many threads and twice as many pieces each 15.4)
         const uint32_t pieces = n * std::max(p.cache.dim, p.cache.vdim) / kPiece, threads = std::min(kThreads, (pieces + 63) / 64 * 64);
-        return pieces <= 2 * kThreads ? on("cache append launch", cache_append_kernel<T, 2>, grid, dim3(threads), p, touched)
-                                      : on("cache append launch", cache_append_kernel<T, 8>, grid, dim3(threads), p, touched);
+        return pieces <= kThreads ? on("cache append launch", cache_append_kernel<T, 1>, grid, dim3(threads), p, touched)
+                                      : on("cache append launch", cache_append_kernel<T, 4>, grid, dim3(threads), p, touched);
     });
 }
 
 int load_cache_append_kernels() {
     hipFuncAttributes a;
-    CG_HIP(hipFuncGetAttributes(&a, reinterpret_cast<const void *>(cache_append_kernel<float, 2>)));
+    CG_HIP(hipFuncGetAttributes(&a, reinterpret_cast<const void *>(cache_append_kernel<float, 1>)));
     return CG_OK;
 }
 
