@@ -124,14 +124,16 @@ size_t shape_cache_attention(CacheAttentionPlan *p) {
     // read (a step of all units: 1.3 us, or with the waves sharing rows 5, at 4.7 TB/s).  768 workgroups for 512 places take as long as 1024:
     // a portion of 3 x 500 rows, 144 groups, took 111 us cut in three, join included, 126 in four, 109 in seven.
     const uint64_t groups = (uint64_t)p->bgs * p->row_blocks;
-    const uint64_t seen = p->window ? std::min<uint64_t>(p->cache.capacity, p->window + p->batch.tokens) : p->cache.capacity, tiles = seen / kTile;
-    const uint32_t least = p->rows_by_wave ? kLeastTilesRows : kLeastTilesShared, step = p->rows_by_wave ? 1 : kWavesOfAttention;
+    const uint64_t C = p->cache.capacity; // what a block of rows sees of it, at most
+    const uint64_t tiles = (p->window ? std::min(C, std::min<uint64_t>(C, p->window) + std::min(p->batch.tokens, group / p->rep + 1)) : C) / kTile;
+    const uint32_t step = p->rows_by_wave ? 1 : kWavesOfAttention;
     const uint64_t joined = (uint64_t)p->bgs * p->rows * p->cache.vdim * 8 * 8 / (p->rows_by_wave ? 6000000 : 24000000); // eighths of a step, for each part
-    const uint64_t most = std::max<uint64_t>(1, std::min<uint64_t>(tiles / least, kMostParts));
+    const uint64_t most = std::max<uint64_t>(1, std::min<uint64_t>(tiles / kLeastTiles, kMostParts));
+    const uint64_t by_row = (uint64_t)p->bgs * p->rows / 160; // the join of more than a few parts, a workgroup for each row: 2048 in 3 us
     uint64_t best = ~0ull;
     p->splits = 1;
     for (uint64_t s = 1; s <= most && groups * (s - 1) < 4 * 512; s++) {
-        const uint64_t cost = 8 * ((groups * s + 511) / 512 * ((tiles + s * step - 1) / (s * step) + 2)) + (s > 1 ? 16 + s * joined : 0);
+        const uint64_t cost = 8 * ((groups * s + 511) / 512 * ((tiles + s * step - 1) / (s * step) + 2)) + (s > 1 ? 16 + s * joined : 0) + (s > kFewParts ? by_row : 0);
         if (cost < best) {
             best = cost;
             p->splits = (uint32_t)s;
