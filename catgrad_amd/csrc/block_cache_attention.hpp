@@ -18,11 +18,13 @@
 // what one 16-bit float does, without the widening of keys: four prompts of 2048 tokens of 16 heads of 128, 84 us against 89).  A block's scale multiplies the scores in 32 bits.  Weights are exp2(score - m + 8) <= 2^15
 // with m the running maximum, which moves only where a score is 7 or more above it (most tiles move none: then nothing is
 // rescaled), as one 16-bit float (2^-12) or two (2^-23), and so is their sum, by the same instruction from ones.
-// Totals are in units of a value block's scale, the codes' own scales being applied as they are widened: exact up to 2^-15 of the
-// unit.  A tile whose scale is larger, or smaller than that, has the totals rescaled to its own (most tiles have none); one whose blocks
-// of 16 or 32 positions lie farther apart is taken a block at a time.  With 16-bit results the instruction adds to the totals
-// itself.  It cuts its sums off, a thousand times for 32000 positions: 2^-15, which such results do not see; with 32-bit results the product of
-// a tile starts from zero and is added by a vector instruction.
+// Totals are in units of a scale 2^unit.  Where many rows have 16-bit results and all value blocks that a workgroup's rows see have scales within
+// 2^15 of each other (they are looked over in front: ScaleRange), the unit is the largest of them, codes are widened times their scale in it, which is exact, and
+// the instruction adds to the totals itself.  It cuts its sums off, a thousand times for 32000 positions: 2^-15, which such results do not see.
+// Else the products of a tile start from zero, in units of the tile's largest scale, and a vector instruction adds them to totals whose unit is the largest scale
+// so far, times the one in units of the other: the unit only rises, so that no total grows beyond its sum of weights times codes, and a block of zeros, whose scale is
+// the smallest, adds zeros.  A tile whose blocks of 16 or 32 positions lie farther than 2^15 apart is taken a block at a time.  (Prompts of 4 x 2048 tokens, bf16, 16 heads of 128:
+// 87 us, the second way 96.)
 //
 // Positions that a row does not see: their weights are set to zero, and since zero times NaN is NaN, a tile that not all rows
 // see whole has its NaN codes of values taken out, and put back into the totals of the rows that do see them.
@@ -45,19 +47,19 @@ typedef short short2v __attribute__((ext_vector_type(2)));
 constexpr uint32_t kTile = 64;           // positions of a wave's tile
 constexpr uint32_t kWavesOfAttention = 4;
 constexpr float kNoMaximum = -3.0e38f;   // of a row that has seen nothing
-// A code times 2^-15 is exact as a 16-bit float (whole multiples of 2^-9, 2^-24); totals of 2^41 units times 2^80 are finite.
-constexpr int kExact = 15, kMostDown = 80;
+constexpr int kExact = 15; // a code times 2^-15 is exact as a 16-bit float (whole multiples of 2^-9, 2^-24)
 // The fewest tiles worth a part of their own: of a token behind 8000 12.9 us, with eight 14.4; a prompt of 1024 tokens of nine heads 23 us, with eight 34.
 constexpr uint32_t kLeastTiles = 4;
 
 // The positions that rows of the tokens s0 .. s1 of a sequence see, cut into at most `splits` parts of whole tiles.
 struct KeyRange {
-    uint32_t first_tile, end_tile, parts, each;
+    uint32_t end, first_tile, end_tile, parts, each;
 };
 __device__ __forceinline__ KeyRange key_range(const CacheAttentionPlan &p, uint64_t held, uint32_t s0, uint32_t s1) {
     const uint64_t C = p.cache.capacity, end = min(held + s1 + 1, C), q0 = held + s0 + 1;
     const uint64_t lo = p.window && q0 > p.window ? min(q0 - p.window, end) : 0;
     KeyRange r;
+    r.end = (uint32_t)end;
     r.first_tile = (uint32_t)(lo / kTile);
     r.end_tile = (uint32_t)((end + kTile - 1) / kTile);
     const uint32_t n = r.end_tile - r.first_tile;
@@ -100,7 +102,6 @@ __device__ __forceinline__ uint32_t quads_max(uint32_t x) {
 template <class T, int NL, int RT, bool CUT = false> struct AttentionWave {
     static_assert(!CUT || NL == 2, "");
     static constexpr int kPieces = sizeof(T) == 4 ? 2 : 1, NV = CUT ? 6 : 4 * NL, kSteps = CUT ? 3 : 2 * NL;
-    static constexpr bool kTotals = kPieces == 1; // the instruction adds to the totals itself
 
     // Queries as codes, for the instructions that take both operands as such.
     static constexpr bool kCodes = std::is_same<T, __bf16>::value && NL >= 2;
@@ -115,8 +116,9 @@ template <class T, int NL, int RT, bool CUT = false> struct AttentionWave {
     float row_factor[RT];
     uint32_t begin[RT], seen_by[RT]; // the lane's rows see seen_by positions from begin on
     int all_from, all_to, any_from, any_to; // positions that all of the wave's rows see, that any does
-    // Totals: sums of weight * value in units of 2^unit.  sums: of the weights, by the same instruction from ones.
-    float4v total[RT][NV], sums[RT];
+    // Totals: sums of weight * value in units of 2^unit.  sums: of the weights, by the same instruction from ones; the first counts.
+    float4v total[RT][NV];
+    float4v sums[RT];
     float maximum[RT];
     int unit = kLowestScale;
     // of the tile at hand
@@ -208,7 +210,7 @@ template <class T, int NL, int RT, bool CUT = false> struct AttentionWave {
                 any_to = max(any_to, last);
             }
             maximum[rt] = kNoMaximum;
-            sums[rt] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+            sums[rt] = {};
 #pragma unroll
             for (int v = 0; v < NV; v++) total[rt][v] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
         }
@@ -333,7 +335,7 @@ template <class T, int NL, int RT, bool CUT = false> struct AttentionWave {
             for (int rt = 0; rt < RT; rt++) {
                 const float m = fmaxf(maximum[rt], quads_max(largest[rt])), down = __builtin_amdgcn_exp2f(maximum[rt] - m);
                 maximum[rt] = m;
-                sums[rt] *= down;
+                sums[rt][0] *= down;
 #pragma unroll
                 for (int v = 0; v < NV; v++) total[rt][v] *= down;
             }
@@ -350,8 +352,9 @@ template <class T, int NL, int RT, bool CUT = false> struct AttentionWave {
         }
     }
 
-    // out^T += V^T weights^T; values(v): the codes, without NaN from the call of clean() on; vs: the scale of the lane's block
-    template <class V, class C> __device__ __forceinline__ void products(float vs, V &&values, C &&clean) {
+    // out^T += V^T weights^T; values(v): the codes, without NaN from the call of clean() on; vs: the scale of the lane's block.  DIRECT: the
+    // instruction adds to the totals, in whose unit all of the tile's codes are exact.
+    template <bool DIRECT, class V, class C> __device__ __forceinline__ void products(float vs, V &&values, C &&clean) {
         // NaN among the values of a tile that not every row sees whole
         if (masked) {
             uint32_t found = 0;
@@ -384,20 +387,6 @@ template <class T, int NL, int RT, bool CUT = false> struct AttentionWave {
                 clean();
             }
         }
-        // the value blocks' scales: of the lane's block, the largest and the smallest of the tile
-        int e = scale_exponent(vs), largest_e, smallest_e;
-        if (p.cache.block_log2 < 6) {
-            const bool seen = mine + 15 >= any_from && mine <= any_to; // (a block that no row sees counts for nothing: its scale may be anything)
-            const int none = -1000;
-            largest_e = quads_max(seen ? e : none);
-            smallest_e = -quads_max(seen ? -e : none);
-            if (largest_e == none) largest_e = smallest_e = kLowestScale;
-            e = seen ? e : largest_e;
-        } else {
-            largest_e = smallest_e = e;
-        }
-        largest_e = __builtin_amdgcn_readfirstlane(largest_e);
-        smallest_e = __builtin_amdgcn_readfirstlane(smallest_e);
         half8v w[RT][kPieces][2];
         const half8v ones = {1, 1, 1, 1, 1, 1, 1, 1};
 #pragma unroll
@@ -409,27 +398,16 @@ template <class T, int NL, int RT, bool CUT = false> struct AttentionWave {
                 w[rt][0][i / 8][i % 8] = h;
                 if (kPieces == 2) w[rt][kPieces - 1][i / 8][i % 8] = (_Float16)(x - (float)h);
             }
-            float4v s = kTotals ? sums[rt] : float4v{0.0f, 0.0f, 0.0f, 0.0f};
+            float4v s = DIRECT ? sums[rt] : float4v{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int piece = kPieces - 1; piece >= 0; piece--)
 #pragma unroll
                 for (int st = 0; st < 2; st++) s = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, w[rt][piece][st], s, 0, 0, 0);
-            sums[rt] = kTotals ? s : sums[rt] + s;
+            if (DIRECT) sums[rt] = s;
+            else sums[rt][0] += s[0];
         }
-        const int passes = largest_e - smallest_e > kExact ? 4 : 1; // (the same for all lanes of a wave)
-        for (int pass = 0; pass < passes; pass++) {
-            asm volatile("" ::: "memory");
-            const int wanted = passes > 1 ? __builtin_amdgcn_readlane(e, pass * 16) : largest_e;
-            if (wanted > unit || wanted < unit - kExact) { // the totals in units of this scale
-                const int to = max(wanted, unit - kMostDown);
-                const float by = power_of_two(max(unit - to, -126));
-                unit = to;
-#pragma unroll
-                for (int rt = 0; rt < RT; rt++)
-#pragma unroll
-                    for (int v = 0; v < NV; v++) total[rt][v] *= by;
-            }
-            const float scale = passes == 1 || (int)quad == pass ? power_of_two(max(e - unit, -126)) : 0.0f;
+        // a pass over the tile's values, their codes times the lane's `scale`; by: a unit of its sums in units of the totals
+        auto add = [&](float scale, float by) {
             constexpr int kAhead = 2;
             uint4 codes[NV];
 #pragma unroll
@@ -443,13 +421,47 @@ template <class T, int NL, int RT, bool CUT = false> struct AttentionWave {
                 for (int st = 0; st < 2; st++) a[st] = eight_of(codes[v], st, scale);
 #pragma unroll
                 for (int rt = 0; rt < RT; rt++) {
-                    float4v s = kTotals ? total[rt][v] : float4v{0.0f, 0.0f, 0.0f, 0.0f};
+                    float4v s = DIRECT ? total[rt][v] : float4v{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                     for (int piece = kPieces - 1; piece >= 0; piece--)
 #pragma unroll
                         for (int st = 0; st < 2; st++) s = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[st], w[rt][piece][st], s, 0, 0, 0);
-                    total[rt][v] = kTotals ? s : total[rt][v] + s;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) total[rt][v][i] = DIRECT ? s[i] : fmaf(s[i], by, total[rt][v][i]);
                 }
+            }
+        };
+        int e = scale_exponent(vs); // of the lane's block
+        if constexpr (DIRECT) {
+            asm volatile("" ::: "memory");
+            add(power_of_two(min(max(e - unit, -kExact), 0)), 1.0f); // (a block that no row sees may have any scale: its weights are zero)
+        } else {
+            int largest_e, smallest_e; // of the tile
+            if (p.cache.block_log2 < 6) {
+                const bool seen = mine + 15 >= any_from && mine <= any_to; // (a block that no row sees counts for nothing: its scale may be anything)
+                const int none = -1000;
+                largest_e = quads_max(seen ? e : none);
+                smallest_e = -quads_max(seen ? -e : none);
+                if (largest_e == none) largest_e = smallest_e = kLowestScale;
+                e = seen ? e : largest_e;
+            } else {
+                largest_e = smallest_e = e;
+            }
+            largest_e = __builtin_amdgcn_readfirstlane(largest_e);
+            smallest_e = __builtin_amdgcn_readfirstlane(smallest_e);
+            const int passes = largest_e - smallest_e > kExact ? 4 : 1; // (the same for all lanes of a wave)
+            for (int pass = 0; pass < passes; pass++) {
+                asm volatile("" ::: "memory");
+                const int wanted = passes > 1 ? __builtin_amdgcn_readlane(e, pass * 16) : largest_e; // the sums' unit
+                if (wanted > unit) { // the totals in the same
+                    const float by = power_of_two(max(unit - wanted, -126));
+                    unit = wanted;
+#pragma unroll
+                    for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+                        for (int v = 0; v < NV; v++) total[rt][v] *= by;
+                }
+                add(passes == 1 || (int)quad == pass ? power_of_two(max(e - wanted, -126)) : 0.0f, power_of_two(max(wanted - unit, -126)));
             }
         }
     }
@@ -517,6 +529,31 @@ struct AttentionShare {
     }
 };
 
+// The exponents of the value blocks of a workgroup's tiles that its rows see, looked over by each of its waves.
+struct ScaleRange {
+    int largest = kLowestScale, smallest = kHighestScale;
+    __device__ __forceinline__ void look(const CacheAttentionPlan &p, const float *v_scale, const AttentionShare &my) {
+        const uint32_t n = p.cache.block_log2, end = min(my.end_tile * kTile, my.range.end); // (blocks behind range.end may have any scale)
+        for (uint32_t j = (my.tile * kTile >> n) + (threadIdx.x & 63); j << n < end; j += 64) {
+            const int e = scale_exponent(v_scale[j]);
+            largest = max(largest, e);
+            smallest = min(smallest, e);
+        }
+    }
+    // Whether codes are exact in units of the largest.
+    __device__ __forceinline__ bool near(int *unit) {
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) {
+            largest = max(largest, __shfl_xor(largest, o));
+            smallest = min(smallest, __shfl_xor(smallest, o));
+        }
+        const int l = __builtin_amdgcn_readfirstlane(largest);
+        if (l - __builtin_amdgcn_readfirstlane(smallest) > kExact) return false;
+        *unit = l;
+        return true;
+    }
+};
+
 // Few rows: the waves of a workgroup have the same rows, take their tiles in turns, codes straight to registers, and add their results up
 // in LDS.  Bound by memory: a token each of 32 sequences behind 16300 (bf16, 32 heads of 128 on 8, 1.07 GB) 160 us, 6.7 TB/s; one behind 131000
 // (f32, 268 MB) 51 us, 5.2 TB/s.
@@ -579,11 +616,11 @@ template <class T, int NL, int RT> __global__ __launch_bounds__(64 * kWavesOfAtt
         const float ks = ks_now;
         if (more) ask_keys(tile + kWavesOfAttention); // (into the registers that the products have read)
         w.weigh(ks);
-        w.products(vs_now, [&](int v) { return v_now[v]; },
-                   [&] {
+        w.template products<false>(vs_now, [&](int v) { return v_now[v]; },
+                                   [&] {
 #pragma unroll
-                       for (int v = 0; v < NV; v++) v_now[v] = without_nan(v_now[v]);
-                   });
+                                       for (int v = 0; v < NV; v++) v_now[v] = without_nan(v_now[v]);
+                                   });
         if (more) ask_values(tile + kWavesOfAttention);
     }
     w.end_tiles();
@@ -627,6 +664,7 @@ template <class T, int NL, int RT, bool CUT = false> __global__ __launch_bounds_
     constexpr int NV = Wave::NV;
     constexpr int kKeys = 4 * NL, kCodes = kKeys + NV; // 1 KB pieces of a tile, of which each wave asks for some
     constexpr bool kOwnCopy = NL <= 2; // (LDS for two workgroups on a compute unit)
+    constexpr bool kMayAdd = sizeof(T) == 2; // the instruction may add to the totals
     extern __shared__ float lds_dyn[];
     lds_char *const lds = (lds_char *)lds_dyn;
     AttentionShare my;
@@ -646,7 +684,7 @@ template <class T, int NL, int RT, bool CUT = false> __global__ __launch_bounds_
 #pragma unroll
     for (int l = 0; l < NL; l++) key_lane[l] = w.key_lane(l);
     const uint32_t value_lane = w.value_lane();
-    auto ask = [&](uint32_t t, uint32_t place) { // the first two waves ask for keys, the others for values
+    auto ask = [&](uint32_t t, uint32_t place) __attribute__((always_inline)) { // the first two waves ask for keys, the others for values
         auto into = [&](uint32_t i, const uint8_t *from) {
             __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from,
                                              (__attribute__((address_space(3))) void *)(lds + (place * kCodes + i) * 1024), 16, 0, 0);
@@ -671,6 +709,8 @@ template <class T, int NL, int RT, bool CUT = false> __global__ __launch_bounds_
         ks_next = k_scale[w.block_of(t)];
         vs_next = v_scale[w.block_of(t)];
     };
+    ScaleRange scales;
+    if (kMayAdd) scales.look(p, v_scale, my);
     uint32_t from = 0, to = 0; // tiles that the wave's rows see
     typename Wave::Queries x;
     if (w.row0 < my.R) w.ask_rows(x); // (in front of the tile: they are wanted first)
@@ -680,45 +720,54 @@ template <class T, int NL, int RT, bool CUT = false> __global__ __launch_bounds_
         from = (uint32_t)max(w.any_from, 0) / kTile;
         to = w.any_to < 0 ? 0 : (uint32_t)w.any_to / kTile + 1;
     }
-    for (uint32_t t = my.tile; t < my.end_tile; t++) {
-        const uint32_t place = (t - my.tile) & 1;
-        asm volatile("" ::: "memory");
-        __builtin_amdgcn_s_waitcnt(0x0070); // vmcnt(0) lgkmcnt(0): this wave's part of the tile is in LDS, and it has read the one before
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        const float ks = ks_next, vs = vs_next;
-        if (t + 1 < my.end_tile) ask(t + 1, place ^ 1);
-        if (t < from || t >= to) continue;
-        const lds_char *const codes = lds + place * kCodes * 1024 + lane * 16;
-        auto piece = [&](int n) {
-            typedef uint32_t u4 __attribute__((ext_vector_type(4)));
-            const u4 v = *reinterpret_cast<const __attribute__((address_space(3))) u4 *>(codes + n * 1024);
-            return make_uint4(v[0], v[1], v[2], v[3]);
-        };
-        w.scores(t, [&](int kt, int l) { return piece(kt * NL + l); });
-        w.weigh(ks);
-        // codes without NaN go to memory of the wave's own (each lane reads what it wrote), so that what the products read is one address
-        // either way: a choice at every piece would keep them from being asked for ahead
-        const lds_char *values_at = codes + kKeys * 1024;
-        bool clean = false;
-        auto value = [&](int v) {
-            typedef uint32_t u4 __attribute__((ext_vector_type(4)));
-            const u4 x = *reinterpret_cast<const __attribute__((address_space(3))) u4 *>(values_at + v * 1024);
-            return make_uint4(x[0], x[1], x[2], x[3]);
-        };
-        w.products(vs, [&](int v) { return !kOwnCopy && clean ? without_nan(value(v)) : value(v); },
-                   [&] {
-                       clean = true;
-                       if (!kOwnCopy) return;
-                       lds_char *const own = lds + (2 * kCodes + wave * NV) * 1024 + lane * 16;
+    const bool near = kMayAdd && scales.near(&w.unit);
+    auto walk = [&](auto direct) __attribute__((always_inline)) {
+        for (uint32_t t = my.tile; t < my.end_tile; t++) {
+            const uint32_t place = (t - my.tile) & 1;
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_s_waitcnt(0x0070); // vmcnt(0) lgkmcnt(0): this wave's part of the tile is in LDS, and it has read the one before
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            const float ks = ks_next, vs = vs_next;
+            if (t + 1 < my.end_tile) ask(t + 1, place ^ 1);
+            if (t < from || t >= to) continue;
+            const lds_char *const codes = lds + place * kCodes * 1024 + lane * 16;
+            auto piece = [&](int n) {
+                typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+                const u4 v = *reinterpret_cast<const __attribute__((address_space(3))) u4 *>(codes + n * 1024);
+                return make_uint4(v[0], v[1], v[2], v[3]);
+            };
+            w.scores(t, [&](int kt, int l) { return piece(kt * NL + l); });
+            w.weigh(ks);
+            // codes without NaN go to memory of the wave's own (each lane reads what it wrote), so that what the products read is one address
+            // either way: a choice at every piece would keep them from being asked for ahead
+            const lds_char *values_at = codes + kKeys * 1024;
+            bool clean = false;
+            auto value = [&](int v) {
+                typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+                const u4 x = *reinterpret_cast<const __attribute__((address_space(3))) u4 *>(values_at + v * 1024);
+                return make_uint4(x[0], x[1], x[2], x[3]);
+            };
+            w.template products<decltype(direct)::value>(vs, [&](int v) { return !kOwnCopy && clean ? without_nan(value(v)) : value(v); },
+                       [&] {
+                           clean = true;
+                           if (!kOwnCopy) return;
+                           lds_char *const own = lds + (2 * kCodes + wave * NV) * 1024 + lane * 16;
 #pragma unroll
-                       for (int v = 0; v < NV; v++) {
-                           typedef uint32_t u4 __attribute__((ext_vector_type(4)));
-                           const uint4 x = without_nan(value(v));
-                           *reinterpret_cast<__attribute__((address_space(3))) u4 *>(own + v * 1024) = u4{x.x, x.y, x.z, x.w};
-                       }
-                       values_at = own;
-                   });
+                           for (int v = 0; v < NV; v++) {
+                               typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+                               const uint4 x = without_nan(value(v));
+                               *reinterpret_cast<__attribute__((address_space(3))) u4 *>(own + v * 1024) = u4{x.x, x.y, x.z, x.w};
+                           }
+                           values_at = own;
+                       });
+        }
+    };
+    if constexpr (kMayAdd) {
+        if (near) walk(std::true_type{});
+        else walk(std::false_type{});
+    } else {
+        walk(std::false_type{});
     }
     __builtin_amdgcn_s_waitcnt(0x0070); // no load may write LDS that another workgroup gets
     if (w.row0 >= my.R) return;

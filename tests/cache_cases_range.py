@@ -1,0 +1,56 @@
+"""Attention over values whose blocks' scales lie far from each other, at the edges of what a scale, a total and a sum of weights can hold.
+Tolerances: see cache_cases.py."""
+import numpy as np
+
+from cache_cases import Cache, append, run_attend
+
+# Few rows are taken by four waves, a tile of 64 positions each in turn; many by waves that walk all tiles, cut into parts of four or more.
+FEW, MANY = 256, 64
+FORMS = {  # dtype, tokens, heads (one of keys and values), dim, vdim, positions that lie in one wave's tile or tiles before its next
+    "few_f32": ("f32", 1, 2, 64, 64, FEW), "few_bf16": ("bf16", 1, 2, 128, 128, FEW), "few_f16": ("f16", 2, 3, 80, 96, FEW),
+    "few_f32_of_256": ("f32", 1, 1, 256, 256, FEW), "few_bf16_20_rows": ("bf16", 10, 2, 64, 64, FEW),
+    "many_f32": ("f32", 40, 1, 64, 64, MANY), "many_bf16": ("bf16", 20, 2, 128, 128, MANY), "many_f16": ("f16", 35, 1, 64, 128, MANY),
+    "many_f32_of_96": ("f32", 40, 1, 96, 80, MANY), "many_bf16_of_96": ("bf16", 40, 1, 80, 96, MANY), "many_bf16_of_256": ("bf16", 40, 1, 256, 256, MANY),
+}
+
+
+def values_by(rng, V, sizes, each):
+    """Values of `each` positions of each of the sizes, from half of it to all of it; size 0: zeros."""
+    x = np.concatenate([np.full((each, 1), float(s)) for s in sizes])
+    return (x * rng.uniform(0.5, 1.0, (len(x), V)))[None]
+
+
+def attend_over(lib, device, form, block, v, what, q=None, k=None, **how):
+    dtype, S, H, D, V, _ = FORMS[form]
+    rng = np.random.default_rng(len(what))
+    T = v.shape[1]
+    cache = Cache(device, 1, 1, D, V, -(-T // block) * block, block)
+    append(lib, device, cache, "f32", [0], [T], rng.standard_normal((1, T, D)) * 0.5 if k is None else k, v)
+    return run_attend(lib, device, cache, dtype, [T - S], [S], rng.standard_normal((1, S, H * D)) * 0.5 if q is None else q, H, what=f"{what} {form} {block}", **how)
+
+
+ZEROS = [[1, 0, 0], [1, 0, 0, 1], [1] + [0] * 11 + [1], [0, 0, 1, 0, 0, 0], [0] * 4, [1, 2.0 ** -100, 2.0 ** -100], [1, 2.0 ** -30, 2.0 ** -60, 2.0 ** -90, 2.0 ** -110, 1]]
+
+
+def run_zeros(lib, device, form, block):
+    """Values of one, then blocks of zeros or of next to nothing: a block of zeros has the smallest scale that there is."""
+    rng = np.random.default_rng(block)
+    V, tiles = FORMS[form][4], FORMS[form][5]
+    for sizes in ZEROS:
+        for each in {max(tiles, block), block}:  # from tile to tile, and within a tile
+            attend_over(lib, device, form, block, values_by(rng, V, sizes * (64 // block if each < 64 else 1), each), f"{sizes} of {each}")
+
+
+def run_between(lib, device, form, block):
+    """A tile of blocks up to 15 exponents apart behind one whose scale is up to 15 exponents larger than theirs; the weights lie on its smallest block."""
+    dtype, S, H, D, V, tiles = FORMS[form]
+    rng = np.random.default_rng(block)
+    top = 2.0 ** (14 if dtype == "f16" else 2)
+    for near, far in ((-15, -30), (-15, -29), (-8, -20), (-1, -16), (-16, -31), (0, -15)):
+        sizes = np.full(2 * tiles + 64, top)
+        sizes[tiles:] = top * 2.0 ** near
+        sizes[2 * tiles - block: 2 * tiles] = sizes[-block:] = top * 2.0 ** far
+        v = sizes[None, :, None] * rng.uniform(0.5, 1.0, (1, len(sizes), V))
+        k = rng.standard_normal((1, len(sizes), D)) * 0.1
+        k[:, 2 * tiles - block: 2 * tiles] += 1.0
+        attend_over(lib, device, form, block, v, f"{near} {far}", q=np.full((1, S, H * D), 100.0 / D), k=k, scale=1.0)

@@ -1,0 +1,18 @@
+"""Attention over values at the edges of what scales and totals hold, on the HIP library."""
+import pytest
+
+import cache_cases_range as E
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("block", [16, 32, 64, 128])
+@pytest.mark.parametrize("form", list(E.FORMS))
+def test_zeros(hip, form, block):
+    E.run_zeros(hip._lib, "cuda", form, block)
+
+
+@pytest.mark.parametrize("block", [16, 32])
+@pytest.mark.parametrize("form", list(E.FORMS))
+def test_between(hip, form, block):
+    E.run_between(hip._lib, "cuda", form, block)
