@@ -327,7 +327,7 @@ template <class T, int NL, int RT, bool CUT = false> struct AttentionWave {
 #pragma unroll
                 for (int i = 0; i < 16; i++) m = fmaxf(m, score[rt][i / 4][i % 4]);
             }
-            largest[rt] = m * factor[rt];
+            largest[rt] = m == -INFINITY ? m : m * factor[rt]; // (a block that nobody has begun may have any scale: a negative one would make this infinite)
             moves = moves || largest[rt] > maximum[rt] + 7.0f;
         }
         if (__any(moves)) {

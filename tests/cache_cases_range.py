@@ -54,3 +54,19 @@ def run_between(lib, device, form, block):
         k = rng.standard_normal((1, len(sizes), D)) * 0.1
         k[:, 2 * tiles - block: 2 * tiles] += 1.0
         attend_over(lib, device, form, block, v, f"{near} {far}", q=np.full((1, S, H * D), 100.0 / D), k=k, scale=1.0)
+
+
+STALE_SCALES = [-2.0, -2.0 ** 127, -float("inf"), float("inf"), float("nan"), -0.0, -2.0 ** -140]
+
+
+def run_stale_scales(lib, device, form, block):
+    """What memory holds in the place of scales of blocks that nobody has begun does not matter."""
+    dtype, S, H, D, V, _ = FORMS[form]
+    rng = np.random.default_rng(block)
+    for stale in STALE_SCALES:
+        for T in (S + 1, 64 + block, 130):
+            cache = Cache(device, 1, 1, D, V, 320 if block < 128 else 384, block)
+            cache.ks.fill_(stale)
+            cache.vs.fill_(stale)
+            append(lib, device, cache, "f32", [0], [T], rng.standard_normal((1, T, D)), rng.standard_normal((1, T, V)))
+            run_attend(lib, device, cache, dtype, [T - S], [S], rng.standard_normal((1, S, H * D)), H, what=f"{stale} {T} {form} {block}")

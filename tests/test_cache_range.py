@@ -12,3 +12,8 @@ def test_zeros(oracle, form, block):
 @pytest.mark.parametrize("form,block", [("few_bf16_20_rows", 16), ("few_f16", 32)])
 def test_between(oracle, form, block):
     E.run_between(oracle._lib, "cpu", form, block)
+
+
+@pytest.mark.parametrize("form,block", [("few_f32", 16), ("few_f16", 32)])
+def test_stale_scales(oracle, form, block):
+    E.run_stale_scales(oracle._lib, "cpu", form, block)

@@ -16,3 +16,9 @@ def test_zeros(hip, form, block):
 @pytest.mark.parametrize("form", list(E.FORMS))
 def test_between(hip, form, block):
     E.run_between(hip._lib, "cuda", form, block)
+
+
+@pytest.mark.parametrize("block", [16, 32, 64, 128])
+@pytest.mark.parametrize("form", list(E.FORMS))
+def test_stale_scales(hip, form, block):
+    E.run_stale_scales(hip._lib, "cuda", form, block)
