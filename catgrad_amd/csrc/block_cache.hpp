@@ -78,7 +78,7 @@ struct CacheAttentionPlan {
     bool rows_by_wave, two_tiles;     // which kernel: see shape_cache_attention
     uint32_t rows;                    // of a pair, at most: tokens * rep
     FastDiv rep_div, bgs_div, splits_div, heads_div, rows_div, run_div; // heads: of keys and values; run: blocks of rows for a card's units
-    float *parts;                     // splits > 1: [pair][split][row][vdim] and behind them [pair][split][row] {maximum, sum}
+    float *parts;                     // splits > 1: [pair][split][row][vdim] results and behind them [pair][split][row] {maximum, sum of weights}
     float2 *stats;
 };
 // Which kernel and cut a call takes, and the bytes of memory that it needs for the parts' results.

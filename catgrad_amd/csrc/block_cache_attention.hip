@@ -6,7 +6,7 @@
 namespace cg {
 namespace {
 
-// out[row] = sum of the parts' totals over the sum of their sums, each scaled from its own maximum to the largest; rows of a block of
+// out[row] = the mean of the parts' results by their sums of weights, each scaled from its own maximum to the largest; rows of a block of
 // rows that was not cut are there already.
 struct RowToJoin {
     uint32_t parts, b, g, r;
@@ -22,10 +22,9 @@ struct RowToJoin {
         first = (uint64_t)bg * p.splits * p.rows + r;
         return parts > 1;
     }
-    template <class T> __device__ __forceinline__ void store(const CacheAttentionPlan &p, uint32_t vec, const float4v &total, float sum) const {
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    template <class T> __device__ __forceinline__ void store(const CacheAttentionPlan &p, uint32_t vec, const float4v &y4) const {
         const uint32_t s = fastdiv(r, p.rep_div), head = g * p.rep + r - s * p.rep;
-        const float y[4] = {total[0] * inv, total[1] * inv, total[2] * inv, total[3] * inv};
+        const float y[4] = {y4[0], y4[1], y4[2], y4[3]};
         store_elements<T, 4>(static_cast<T *>(p.out) + ((int64_t)b * p.batch.tokens + s) * p.out_pitch + head * p.cache.vdim + vec * 4, y);
     }
 };
@@ -44,24 +43,26 @@ template <class T> __global__ __launch_bounds__(256) void join_few_parts_kernel(
         stats[i] = p.stats[at];
         part[i] = *reinterpret_cast<const float4v *>(p.parts + at * p.cache.vdim + vec * 4);
     }
-    float m = stats[0].x, sum = 0.0f;
+    float m = stats[0].x, sum = 0.0f, weight[kFewParts];
 #pragma unroll
     for (uint32_t i = 1; i < kFewParts; i++) m = fmaxf(m, stats[i].x);
-    float4v total = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (uint32_t i = 0; i < kFewParts; i++) {
-        if (i >= row.parts) continue;
-        const float f = __builtin_amdgcn_exp2f(stats[i].x - m);
-        sum += stats[i].y * f;
-        total += part[i] * f;
+        weight[i] = i < row.parts ? stats[i].y * __builtin_amdgcn_exp2f(stats[i].x - m) : 0.0f;
+        sum += weight[i];
     }
-    row.store<T>(p, vec, total, sum);
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    float4v total = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (uint32_t i = 0; i < kFewParts; i++)
+        if (i < row.parts) total += part[i] * (weight[i] * inv);
+    row.store<T>(p, vec, total);
 }
 
-// Many parts: a workgroup takes a row, its threads the parts' factors first, then channels of some of the parts each.
+// Many parts: a workgroup takes a row, its threads the parts' weights first, then channels of some of the parts each.
 constexpr uint32_t kMostParts = 256;
 template <class T> __global__ __launch_bounds__(256) void join_parts_kernel(CacheAttentionPlan p, uint32_t lanes, uint32_t each, uint32_t group) {
-    __shared__ float factors[kMostParts], reduced[8];
+    __shared__ float weights[kMostParts], reduced[8];
     __shared__ float4v totals[256];
     RowToJoin row;
     if (!row.find(p, blockIdx.x, group)) return; // (the same for all threads)
@@ -72,14 +73,14 @@ template <class T> __global__ __launch_bounds__(256) void join_parts_kernel(Cach
     if (threadIdx.x % 64 == 0) reduced[threadIdx.x / 64] = m;
     __syncthreads();
     m = fmaxf(fmaxf(reduced[0], reduced[1]), fmaxf(reduced[2], reduced[3]));
-    const float f = __builtin_amdgcn_exp2f(mine.x - m);
-    factors[threadIdx.x] = f;
-    float sum = mine.y * f;
+    float sum = mine.y * __builtin_amdgcn_exp2f(mine.x - m);
+    weights[threadIdx.x] = sum;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
     if (threadIdx.x % 64 == 0) reduced[4 + threadIdx.x / 64] = sum;
     __syncthreads();
     sum = reduced[4] + reduced[5] + reduced[6] + reduced[7];
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
     const uint32_t turn = threadIdx.x / lanes, vec = threadIdx.x - turn * lanes; // every `each`-th part
     float4v total = {0.0f, 0.0f, 0.0f, 0.0f};
     if (turn < each) {
@@ -93,14 +94,14 @@ template <class T> __global__ __launch_bounds__(256) void join_parts_kernel(Cach
             }
 #pragma unroll
             for (uint32_t k = 0; k < kAtOnce; k++)
-                if (i0 + k * each < row.parts) total += part[k] * factors[i0 + k * each];
+                if (i0 + k * each < row.parts) total += part[k] * (weights[i0 + k * each] * inv);
         }
     }
     totals[threadIdx.x] = total;
     __syncthreads();
     if (threadIdx.x >= lanes) return;
     for (uint32_t i = 1; i < each; i++) total += totals[i * lanes + threadIdx.x];
-    row.store<T>(p, vec, total, sum);
+    row.store<T>(p, vec, total);
 }
 
 uint32_t rows_of_group(const CacheAttentionPlan &p) {

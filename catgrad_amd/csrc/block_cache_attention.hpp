@@ -465,11 +465,16 @@ template <class T, int NL, int RT, bool CUT = false> struct AttentionWave {
             }
         }
     }
+    // Totals become results: divided first (sums of weights of 2^8 and more, times a value of 2^119, are no 32-bit floats; their quotient is).
     __device__ __forceinline__ void end_tiles() {
 #pragma unroll
-        for (int rt = 0; rt < RT; rt++)
+        for (int rt = 0; rt < RT; rt++) {
+            const float sum = sums[rt][0], inv = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
-            for (int v = 0; v < NV; v++) total[rt][v] *= power_of_two(unit);
+            for (int v = 0; v < NV; v++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) total[rt][v][i] = total[rt][v][i] * inv * power_of_two(unit);
+        }
     }
 
     // The rows' results, or those of one of their parts.
@@ -479,20 +484,18 @@ template <class T, int NL, int RT, bool CUT = false> struct AttentionWave {
         for (int rt = 0; rt < RT; rt++) {
             const uint32_t r = row0 + rt * 16 + col;
             if (r >= R) continue;
-            const float sum = sums[rt][0];
             if (parts == 1) {
-                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
                 const uint32_t head = g * p.rep + r - fastdiv(r, p.rep_div) * p.rep;
                 T *const dst = static_cast<T *>(p.out) + token_of(rt) * p.out_pitch + head * c.vdim + quad * 4;
 #pragma unroll
                 for (int v = 0; v < NV; v++) {
                     if (v * 16 >= (int)c.vdim) continue;
-                    const float y[4] = {total[rt][v][0] * inv, total[rt][v][1] * inv, total[rt][v][2] * inv, total[rt][v][3] * inv};
+                    const float y[4] = {total[rt][v][0], total[rt][v][1], total[rt][v][2], total[rt][v][3]};
                     store_elements<T, 4>(dst + v * 16, y);
                 }
             } else {
                 const uint64_t at = ((uint64_t)(b * c.kv_heads + g) * p.splits + split) * p.rows + r;
-                if (quad == 0) p.stats[at] = make_float2(maximum[rt], sum);
+                if (quad == 0) p.stats[at] = make_float2(maximum[rt], sums[rt][0]);
                 float *const dst = p.parts + at * c.vdim + quad * 4;
 #pragma unroll
                 for (int v = 0; v < NV; v++)
@@ -623,13 +626,14 @@ template <class T, int NL, int RT> __global__ __launch_bounds__(64 * kWavesOfAtt
                                    });
         if (more) ask_values(tile + kWavesOfAttention);
     }
-    w.end_tiles();
-    // the waves' results: of two and two, then of the last two
+    // the waves' totals: of two and two, then of the last two
     __shared__ float4v shared_total[2][RT * NV][64];
     __shared__ float2 shared_stats[2][RT][64];
+    __shared__ int shared_unit[2];
 #pragma unroll
     for (uint32_t half = 2; half >= 1; half /= 2) {
         if (wave >= half && wave < 2 * half) {
+            shared_unit[wave - half] = w.unit;
 #pragma unroll
             for (int rt = 0; rt < RT; rt++) {
                 shared_stats[wave - half][rt][lane] = make_float2(w.maximum[rt], w.sums[rt][0]);
@@ -639,19 +643,24 @@ template <class T, int NL, int RT> __global__ __launch_bounds__(64 * kWavesOfAtt
         }
         __syncthreads();
         if (wave < half) {
+            const int its_unit = shared_unit[wave], unit = max(w.unit, its_unit);
 #pragma unroll
             for (int rt = 0; rt < RT; rt++) {
                 const float2 other = shared_stats[wave][rt][lane];
                 const float m = fmaxf(w.maximum[rt], other.x), mine = __builtin_amdgcn_exp2f(w.maximum[rt] - m), its = __builtin_amdgcn_exp2f(other.x - m);
                 w.maximum[rt] = m;
                 w.sums[rt][0] = w.sums[rt][0] * mine + other.y * its;
+                const float my_part = __builtin_amdgcn_ldexpf(mine, w.unit - unit), its_part = __builtin_amdgcn_ldexpf(its, its_unit - unit);
 #pragma unroll
-                for (int v = 0; v < NV; v++) w.total[rt][v] = w.total[rt][v] * mine + shared_total[wave][rt * NV + v][lane] * its;
+                for (int v = 0; v < NV; v++) w.total[rt][v] = w.total[rt][v] * my_part + shared_total[wave][rt * NV + v][lane] * its_part;
             }
+            w.unit = unit;
         }
         __syncthreads();
     }
-    if (wave == 0) w.store(my.range.parts, my.split);
+    if (wave > 0) return;
+    w.end_tiles();
+    w.store(my.range.parts, my.split);
 }
 
 // Many rows: every wave of a workgroup has rows of its own, and all walk the same tiles, whose codes come straight into LDS, a tile ahead, in

@@ -70,3 +70,21 @@ def run_stale_scales(lib, device, form, block):
             cache.vs.fill_(stale)
             append(lib, device, cache, "f32", [0], [T], rng.standard_normal((1, T, D)), rng.standard_normal((1, T, V)))
             run_attend(lib, device, cache, dtype, [T - S], [S], rng.standard_normal((1, S, H * D)), H, what=f"{stale} {T} {form} {block}")
+
+
+LARGE = [2.0 ** 112, 2.0 ** 119, 448 * 2.0 ** 119]
+
+
+def run_large(lib, device, form, block, positions=200):
+    """Values as large as a cache holds, of which an average is no larger."""
+    dtype, S, H, D, V, _ = FORMS[form]
+    rng = np.random.default_rng(block)
+    for size in LARGE:
+        for low in (1.0, -1.0, 0.5):
+            v = size * (rng.uniform(low, 1.0, (1, positions, V)) if low < 1 else np.ones((1, positions, V)))
+            attend_over(lib, device, form, block, v, f"{size} {low}")
+            attend_over(lib, device, form, block, v, f"{size} {low} equal keys", k=np.ones((1, positions, D)))
+    # the large ones in one part or wave of some
+    v = np.ones((1, positions, V))
+    v[:, positions // 3: positions // 2] = LARGE[-1]
+    attend_over(lib, device, form, block, v, "some large")

@@ -22,3 +22,14 @@ def test_between(hip, form, block):
 @pytest.mark.parametrize("form", list(E.FORMS))
 def test_stale_scales(hip, form, block):
     E.run_stale_scales(hip._lib, "cuda", form, block)
+
+
+@pytest.mark.parametrize("block", [16, 64])
+@pytest.mark.parametrize("form", [f for f in E.FORMS if "_f16" not in f])
+def test_large(hip, form, block):
+    E.run_large(hip._lib, "cuda", form, block)
+
+
+@pytest.mark.parametrize("form,positions", [("few_f32", 4000), ("few_f32", 20000), ("few_bf16", 4000), ("few_bf16", 20000), ("many_bf16", 4000), ("many_f32", 2000)])
+def test_large_in_parts(hip, form, positions):
+    E.run_large(hip._lib, "cuda", form, 64, positions)
