@@ -23,7 +23,8 @@
 // the instruction adds to the totals itself.  It cuts its sums off, a thousand times for 32000 positions: 2^-15, which such results do not see.
 // Else the products of a tile start from zero, in units of the tile's largest scale, and a vector instruction adds them to totals whose unit is the largest scale
 // so far, times the one in units of the other: the unit only rises, so that no total grows beyond its sum of weights times codes, and a block of zeros, whose scale is
-// the smallest, adds zeros.  A tile whose blocks of 16 or 32 positions lie farther than 2^15 apart is taken a block at a time.  (Prompts of 4 x 2048 tokens, bf16, 16 heads of 128:
+// the smallest, adds zeros.  (Scales lie within 2^236 of each other: where a row sees nothing but values 2^126 below those of another row of its wave, its total runs
+// out of the normal numbers, to 2^-157 of the wave's largest scale.)  A tile whose blocks of 16 or 32 positions lie farther than 2^15 apart is taken a block at a time.  (Prompts of 4 x 2048 tokens, bf16, 16 heads of 128:
 // 87 us, the second way 96.)
 //
 // Positions that a row does not see: their weights are set to zero, and since zero times NaN is NaN, a tile that not all rows
@@ -454,14 +455,16 @@ template <class T, int NL, int RT, bool CUT = false> struct AttentionWave {
                 asm volatile("" ::: "memory");
                 const int wanted = passes > 1 ? __builtin_amdgcn_readlane(e, pass * 16) : largest_e; // the sums' unit
                 if (wanted > unit) { // the totals in the same
-                    const float by = power_of_two(max(unit - wanted, -126));
+                    const int down = unit - wanted;
                     unit = wanted;
 #pragma unroll
                     for (int rt = 0; rt < RT; rt++)
 #pragma unroll
-                        for (int v = 0; v < NV; v++) total[rt][v] *= by;
+                        for (int v = 0; v < NV; v++)
+#pragma unroll
+                            for (int i = 0; i < 4; i++) total[rt][v][i] = __builtin_amdgcn_ldexpf(total[rt][v][i], down);
                 }
-                add(passes == 1 || (int)quad == pass ? power_of_two(max(e - wanted, -126)) : 0.0f, power_of_two(max(wanted - unit, -126)));
+                add(passes == 1 || (int)quad == pass ? power_of_two(max(e - wanted, -kExact)) : 0.0f, __builtin_amdgcn_ldexpf(1.0f, wanted - unit));
             }
         }
     }

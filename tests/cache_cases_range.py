@@ -1,8 +1,13 @@
 """Attention over values whose blocks' scales lie far from each other, at the edges of what a scale, a total and a sum of weights can hold.
 Tolerances: see cache_cases.py."""
+import ctypes as C
+
 import numpy as np
 
-from cache_cases import Cache, append, run_attend
+import cache_reference as R
+
+from cache_cases import HALF, TERMS, TYPES, WEIGHT, Cache, Rows, append, check, f64, lengths, off_by, run_attend, stream_of
+from catgrad_amd import _abi as A
 
 # Few rows are taken by four waves, a tile of 64 positions each in turn; many by waves that walk all tiles, cut into parts of four or more.
 FEW, MANY = 256, 64
@@ -88,3 +93,30 @@ def run_large(lib, device, form, block, positions=200):
     v = np.ones((1, positions, V))
     v[:, positions // 3: positions // 2] = LARGE[-1]
     attend_over(lib, device, form, block, v, "some large")
+
+
+def run_rows_apart(lib, device, form, block):
+    """Rows that see nothing but values 2^135 smaller than those that others of their wave see.  A row's total is a 32-bit float in units of the
+    largest scale that its wave has met, and its weights are 2^8 or more at their largest: the total's smallest step, 2^-149 of a unit, is 2^-157 of a result's,
+    and may be lost once for each of the 16 instructions of a tile.  A scale is at most 2^-7 of its block's largest value."""
+    dtype, S, H, D, V, _ = FORMS[form]
+    rng = np.random.default_rng(block)
+    small, large = 2.0 ** -60, 2.0 ** 75
+    v = values_by(rng, V, [small, large], block)
+    q, k, held = rng.standard_normal((1, S, H * D)) * 0.5, rng.standard_normal((1, 2 * block, D)) * 0.5, max(block - (S + 1) // 2, 0)
+    cache = Cache(device, 1, 1, D, V, 2 * block, block)
+    append(lib, device, cache, "f32", [0], [2 * block], k, v)
+    rq, out = Rows(q, dtype, device), Rows(np.zeros((1, S, H * V)), dtype, device)
+    h, c = lengths(device, [held], [S])
+    a = A.CacheAttentionRows(A.TokenBatch(1, S, 0, h.data_ptr(), c.data_ptr()), TYPES[dtype][1], rq.rows.data_ptr(), out.rows.data_ptr(), rq.pitch, out.pitch, H,
+                             cache.struct(), D ** -0.5, 0, None, 0)
+    need = C.c_size_t()
+    check(lib, lib.cg_cache_attention_workspace(a, need))
+    assert need.value == 0  # (one part: so few positions are not cut)
+    check(lib, lib.cg_cache_attention_noalloc(0, a, stream_of(device)))
+    x, y = f64(rq.rows).reshape(S, H, D), f64(out.rows).reshape(S, H, V)
+    keys, values = (t.x for t in cache.heads[0][0])
+    for s in range(S):
+        want, size, terms = R.attend(x[s], held + s, keys, values, D ** -0.5, 0)
+        tol = 2 * (TERMS[dtype] * terms + 2.0 ** -20 + WEIGHT[dtype]) * size + HALF[dtype] * np.abs(want) + 16 * 2.0 ** -157 * 2.0 ** -7 * large
+        off_by(y[s], want, tol, f"{form} {block} row {s}")

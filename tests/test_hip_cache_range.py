@@ -33,3 +33,9 @@ def test_large(hip, form, block):
 @pytest.mark.parametrize("form,positions", [("few_f32", 4000), ("few_f32", 20000), ("few_bf16", 4000), ("few_bf16", 20000), ("many_bf16", 4000), ("many_f32", 2000)])
 def test_large_in_parts(hip, form, positions):
     E.run_large(hip._lib, "cuda", form, 64, positions)
+
+
+@pytest.mark.parametrize("block", [16, 64, 128])
+@pytest.mark.parametrize("form", [f for f in E.FORMS if "_f16" not in f])
+def test_rows_apart(hip, form, block):
+    E.run_rows_apart(hip._lib, "cuda", form, block)
