@@ -20,7 +20,8 @@
 // rescaled), as one 16-bit float (2^-12) or two (2^-23), and so is their sum, by the same instruction from ones.
 // Totals are in units of a scale 2^unit.  Where many rows have 16-bit results and all value blocks that a workgroup's rows see have scales within
 // 2^15 of each other (they are looked over in front: ScaleRange), the unit is the largest of them, codes are widened times their scale in it, which is exact, and
-// the instruction adds to the totals itself.  It cuts its sums off, a thousand times for 32000 positions: 2^-15, which such results do not see.
+// the instruction adds to the totals itself.  It cuts its sums off a little below their last bit: results of 16-bit floats measured 2^-13.6 too small behind 4 million positions in
+// one part, 2^-12 behind 16 million, where half a step is 2^-11; so it does up to kMostTiles tiles.
 // Else the products of a tile start from zero, in units of the tile's largest scale, and a vector instruction adds them to totals whose unit is the largest scale
 // so far, times the one in units of the other: the unit only rises, so that no total grows beyond its sum of weights times codes, and a block of zeros, whose scale is
 // the smallest, adds zeros.  (Scales lie within 2^236 of each other: where a row sees nothing but values 2^126 below those of another row of its wave, its total runs
@@ -48,6 +49,7 @@ typedef short short2v __attribute__((ext_vector_type(2)));
 constexpr uint32_t kTile = 64;           // positions of a wave's tile
 constexpr uint32_t kWavesOfAttention = 4;
 constexpr float kNoMaximum = -3.0e38f;   // of a row that has seen nothing
+constexpr uint32_t kMostTiles = 65536;   // that the instruction adds to totals itself
 constexpr int kExact = 15; // a code times 2^-15 is exact as a 16-bit float (whole multiples of 2^-9, 2^-24)
 // The fewest tiles worth a part of their own: of a token behind 8000 12.9 us, with eight 14.4; a prompt of 1024 tokens of nine heads 23 us, with eight 34.
 constexpr uint32_t kLeastTiles = 4;
@@ -722,7 +724,8 @@ template <class T, int NL, int RT, bool CUT = false> __global__ __launch_bounds_
         vs_next = v_scale[w.block_of(t)];
     };
     ScaleRange scales;
-    if (kMayAdd) scales.look(p, v_scale, my);
+    const bool few_tiles = kMayAdd && my.end_tile <= my.tile + kMostTiles;
+    if (few_tiles) scales.look(p, v_scale, my);
     uint32_t from = 0, to = 0; // tiles that the wave's rows see
     typename Wave::Queries x;
     if (w.row0 < my.R) w.ask_rows(x); // (in front of the tile: they are wanted first)
@@ -732,7 +735,7 @@ template <class T, int NL, int RT, bool CUT = false> __global__ __launch_bounds_
         from = (uint32_t)max(w.any_from, 0) / kTile;
         to = w.any_to < 0 ? 0 : (uint32_t)w.any_to / kTile + 1;
     }
-    const bool near = kMayAdd && scales.near(&w.unit);
+    const bool near = few_tiles && scales.near(&w.unit);
     auto walk = [&](auto direct) __attribute__((always_inline)) {
         for (uint32_t t = my.tile; t < my.end_tile; t++) {
             const uint32_t place = (t - my.tile) & 1;
