@@ -30,7 +30,7 @@ int check_rotation(size_t heads, size_t kv_heads, size_t dim, size_t rot, const 
     return CG_OK;
 }
 
-// Sizes of a cache and of what is done with it; workgroups of the launches stay below 2^24 (2^32 threads).
+// Sizes of a cache and of what is done with it.
 int check_cache(size_t sequences, size_t tokens, size_t kv_heads, size_t dim, size_t vdim, size_t capacity, size_t block, const char *what) {
     if (!cache_dim(dim) || !cache_dim(vdim)) return fail(CG_ERR_UNSUPPORTED, "%s: heads of 16, 32, .. 256 channels", what);
     if (block_log2(block) < 0) return fail(CG_ERR_UNSUPPORTED, "%s: blocks of 16, 32, 64 or 128 positions", what);
@@ -45,6 +45,12 @@ int check_heads(size_t heads, size_t kv_heads, size_t tokens, float scale, const
     if (heads / kv_heads * tokens >= 1u << 24) return fail(CG_ERR_UNSUPPORTED, "%s: too many rows in one call", what);
     if (!std::isfinite(scale)) return fail(CG_ERR_ARG, "%s: the scale is not a finite number", what);
     return CG_OK;
+}
+
+// A launch's threads are fewer than 2^32 (an append's workgroups have up to 512).
+int check_launch(const CacheAppendPlan &p) {
+    const AppendShape s = shape_cache_append(p);
+    return s.groups * s.threads >= 1ull << 32 ? fail(CG_ERR_UNSUPPORTED, "cache append: too many blocks in one call") : CG_OK;
 }
 
 template <class F> int guarded(F &&f) { // (nothing is thrown through the C ABI)
@@ -376,6 +382,7 @@ int cg_block_cache_append(cg_backend *b, const cg_cache_append_args *a, cg_tenso
         if (a->position + (uint64_t)S > c.capacity) return fail(CG_ERR_RANGE, "%s: the cache has no room for the positions", what);
         if (a->v->dims[0] != B || a->v->dims[1] != S) return fail(CG_ERR_SHAPE, "%s: k and v have different tokens", what);
         p.batch = batch_of(B, S, a->position);
+        if (int rc = check_launch(p)) return rc;
         if (int rc = activations(b, h, a->k, B * S, (int64_t)c.kv_heads * c.dim, &p.k, &p.k_pitch, what)) return rc;
         if (int rc = activations(b, h, a->v, B * S, (int64_t)c.kv_heads * c.vdim, &p.v, &p.v_pitch, what)) return rc;
         cg_tensor *o[4] = {};
@@ -506,6 +513,7 @@ int cg_cache_append_noalloc(int device, const cg_cache_append_rows *a, void *str
     if (!a->k || !a->v) return fail(CG_ERR_ARG, "%s: null argument", what);
     if (int rc = pitch_of(a->k_pitch, a->cache.kv_heads * a->cache.dim, &p.k_pitch, what)) return rc;
     if (int rc = pitch_of(a->v_pitch, a->cache.kv_heads * a->cache.vdim, &p.v_pitch, what)) return rc;
+    if (int rc = check_launch(p)) return rc;
     p.k = a->k;
     p.v = a->v;
     OnDevice on(device);

@@ -62,6 +62,12 @@ struct CacheAppendPlan {
     int64_t k_pitch, v_pitch;
     Cache8 cache;
 };
+// The launch of an append: the blocks of a head that it touches at most, and a workgroup's threads.
+struct AppendShape {
+    uint32_t touched, threads;
+    uint64_t groups; // workgroups
+};
+AppendShape shape_cache_append(const CacheAppendPlan &p);
 int launch_cache_append(const LaunchOn &on, cg_dtype dtype, const CacheAppendPlan &p);
 
 struct CacheAttentionPlan {

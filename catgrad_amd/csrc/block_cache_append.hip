@@ -218,18 +218,25 @@ template <class T, int UNITS> __global__ __launch_bounds__(kThreads) void cache_
 
 } // namespace
 
-int launch_cache_append(const LaunchOn &on, cg_dtype dtype, const CacheAppendPlan &p) {
-    const uint32_t n = 1u << p.cache.block_log2;
+AppendShape shape_cache_append(const CacheAppendPlan &p) {
+    const uint32_t n = 1u << p.cache.block_log2, heads = p.cache.kv_heads * 2;
+    if (p.batch.tokens == 1) return {1, 64, (uint64_t)p.batch.sequences * heads};
     const uint32_t touched = std::min(p.cache.capacity / n, (p.batch.tokens + n - 2) / n + 1);
+    // a thread for a piece of a block, up to 512, then up to four of the largest blocks' pieces a thread (2 x 500 tokens, f32, heads of 256 in blocks of 128: 12.0 us;
+    // with half as many threads and twice as many pieces each 15.4)
+    const uint32_t pieces = n * std::max(p.cache.dim, p.cache.vdim) / kPiece;
+    return {touched, std::min(kThreads, (pieces + 63) / 64 * 64), (uint64_t)touched * p.batch.sequences * heads};
+}
+
+int launch_cache_append(const LaunchOn &on, cg_dtype dtype, const CacheAppendPlan &p) {
+    const AppendShape s = shape_cache_append(p);
     return with_element(dtype, [&](auto e) {
         typedef decltype(e) T;
-        if (p.batch.tokens == 1) return on("cache append launch", cache_append_token_kernel<T>, dim3(p.batch.sequences * p.cache.kv_heads * 2), dim3(64), p);
-        const dim3 grid(touched * p.cache.kv_heads * p.batch.sequences * 2);
-        // a thread for a piece of a block, up to 512, then up to four of the largest blocks' pieces a thread (2 x 500 tokens, f32, heads of 256 in blocks of 128: 12.0 us;
-        // with half as many threads and twice as many pieces each 15.4)
-        const uint32_t pieces = n * std::max(p.cache.dim, p.cache.vdim) / kPiece, threads = std::min(kThreads, (pieces + 63) / 64 * 64);
-        return pieces <= kThreads ? on("cache append launch", cache_append_kernel<T, 1>, grid, dim3(threads), p, touched)
-                                      : on("cache append launch", cache_append_kernel<T, 4>, grid, dim3(threads), p, touched);
+        const dim3 grid((uint32_t)s.groups), block(s.threads);
+        if (p.batch.tokens == 1) return on("cache append launch", cache_append_token_kernel<T>, grid, block, p);
+        const uint32_t pieces = (std::max(p.cache.dim, p.cache.vdim) << p.cache.block_log2) / kPiece;
+        return pieces <= kThreads ? on("cache append launch", cache_append_kernel<T, 1>, grid, block, p, s.touched)
+                                  : on("cache append launch", cache_append_kernel<T, 4>, grid, block, p, s.touched);
     });
 }
 
