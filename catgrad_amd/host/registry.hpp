@@ -28,7 +28,13 @@ inline void read_rope_scaling(const Json &j, cg_rotation &r) {
         r.low = bands ? s->at("low_freq_factor").real() : value("beta_slow", 1.0);
         r.high = bands ? s->at("high_freq_factor").real() : value("beta_fast", 32.0);
         r.original = value("original_max_position_embeddings", all ? all->real() : 0.0);
-        if (!bands) r.magnitude = value("attention_factor", 0.0);
+        if (!bands) { // (what else the section may say about its limits and its magnitude is refused, not passed over)
+            const Json *whole = s->find("truncate");
+            r.magnitude = value("attention_factor", 0.0);
+            if (whole && !whole->flag()) throw ConfigError("config: rope_scaling's limits are whole pairs (\"truncate\")");
+            if (r.magnitude == 0.0 && (value("mscale", 0.0) != 0.0 || value("mscale_all_dim", 0.0) != 0.0))
+                throw ConfigError("config: rope_scaling's \"mscale\" is not followed; \"attention_factor\" is");
+        }
     } else {
         throw ConfigError("config: unknown rope_scaling '" + t->str() + "'");
     }
