@@ -6,8 +6,8 @@
 // channel: a thread takes 16 neighbouring positions of a channel, reads them from 16 rows (a wave's lanes take neighbouring
 // channels) and stores them in one piece, together with what the piece held of older positions.  No two workgroups share a byte
 // that either writes.  A block that grew has the rest of its codes rounded anew in a second sweep, which few appends need.
-// Bound by memory: 4 prompts of 2048 tokens (f32, 8 heads of 128, 84 MB) 18.4 us, 4.6 TB/s; short ragged ones by latency: 7 of up to
-// 301 tokens (f16, 6 heads of 80 / 96, 6.7 MB) 6.4 us.
+// Bound by memory: 4 prompts of 2048 tokens (f32, 8 heads of 128, 84 MB) 19.1 us, 4.4 TB/s.  With 16-bit elements (50 MB, and 8 MB of codes
+// that are read in front of being written) 19.0 us as well: 3.1 TB/s, what bounds that is not known.  Short ragged ones are bound by latency: 7 of up to 301 tokens (f16, 6 heads of 80 / 96, 6.7 MB) 6.9 us.
 #include "block_cache.hpp"
 #include "device_utils.hpp"
 

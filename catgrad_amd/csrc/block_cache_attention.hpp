@@ -17,7 +17,8 @@
 // where they lie 2^14 below the row's largest (there to 2^-22 of it): then the instruction takes the keys' codes as they are (v_mfma_scale_f32_16x16x128_f8f6f4, at twice the rate, so that the two cost
 // what one 16-bit float does, without the widening of keys: four prompts of 2048 tokens of 16 heads of 128, 84 us against 89).  A block's scale multiplies the scores in 32 bits.  Weights are exp2(score - m + 8) <= 2^15
 // with m the running maximum, which moves only where a score is 7 or more above it (most tiles move none: then nothing is
-// rescaled), as one 16-bit float (2^-12) or two (2^-23), and so is their sum, by the same instruction from ones.
+// rescaled), as one 16-bit float (2^-12) or two (2^-23), and so is their sum, by the same instruction from ones.  Either way a weight is off by up to
+// 2^-33 of its row's largest, and may be zero below that.
 // Totals are in units of a scale 2^unit.  Where many rows have 16-bit results and all value blocks that a workgroup's rows see have scales within
 // 2^15 of each other (they are looked over in front: ScaleRange), the unit is the largest of them, codes are widened times their scale in it, which is exact, and
 // the instruction adds to the totals itself.  It cuts its sums off a little below their last bit: results of 16-bit floats measured 2^-13.6 too small behind 4 million positions in
@@ -101,7 +102,7 @@ __device__ __forceinline__ uint32_t quads_max(uint32_t x) {
 
 // What a wave knows of its rows, and does with a tile.  RT: 16-row groups; NL: 64-channel pieces of a head.  CUT: heads of at most 96
 // channels, whose second 64 are two pieces of 16 (in 16-bit floats one step of the products, of which the quads take eight channels each) and whose values
-// are six groups of 16, not eight (only where rows are many: few are bound by memory).  Portions of 3 x 500 tokens behind texts, f32 heads of 96 / 80: 86 us, 102 without.
+// are six groups of 16, not eight (only where rows are many: few are bound by memory).  Portions of 3 x 500 tokens behind texts, f32 heads of 96 / 80: 86 us where it was 102.
 template <class T, int NL, int RT, bool CUT = false> struct AttentionWave {
     static_assert(!CUT || NL == 2, "");
     static constexpr int kPieces = sizeof(T) == 4 ? 2 : 1, NV = CUT ? 6 : 4 * NL, kSteps = CUT ? 3 : 2 * NL;
@@ -563,7 +564,7 @@ struct ScaleRange {
 };
 
 // Few rows: the waves of a workgroup have the same rows, take their tiles in turns, codes straight to registers, and add their results up
-// in LDS.  Bound by memory: a token each of 32 sequences behind 16300 (bf16, 32 heads of 128 on 8, 1.07 GB) 160 us, 6.7 TB/s; one behind 131000
+// in LDS.  Bound by memory: a token each of 32 sequences behind 16300 (bf16, 32 heads of 128 on 8, 1.07 GB, of which two passes find a sixth in the card's cache) 162 us, 6.6 TB/s; one behind 131000
 // (f32, 268 MB) 51 us, 5.2 TB/s.
 template <class T, int NL, int RT> __global__ __launch_bounds__(64 * kWavesOfAttention, NL * RT > 2 ? 1 : 2) void cache_attention_kernel(CacheAttentionPlan p) {
     typedef AttentionWave<T, NL, RT> Wave;
@@ -669,8 +670,9 @@ template <class T, int NL, int RT> __global__ __launch_bounds__(64 * kWavesOfAtt
 }
 
 // Many rows: every wave of a workgroup has rows of its own, and all walk the same tiles, whose codes come straight into LDS, a tile ahead, in
-// the order in which the lanes take them.  Bound by the vector instructions between the products (widening codes, weights): four prompts of 2048 tokens (bf16,
-// 16 heads of 128 on 8, 69 GFLOP) 83 us in a run of calls, matrix pipes busy for 29 % of the cycles, vector instructions for 43 %; of the 31 us of a workgroup of 9 to 16
+// the order in which the lanes take them.  Bound by what waits for what: scores, their maximum, exponentials and products follow each other in each wave, and the two waves of a
+// SIMD cover that in part.  Four prompts of 2048 tokens (bf16,
+// 16 heads of 128 on 8, 69 GFLOP) 82 to 84 us in a run of calls, matrix pipes busy for 29 % of the cycles, vector instructions for 42 %; of the 31 us of a workgroup of 9 to 16
 // tiles 6 to 8 are its beginning and end.  128 rows share what a tile costs to fetch; with 16 a wave the widening would be done twice as often.
 template <class T, int NL, int RT, bool CUT = false> __global__ __launch_bounds__(64 * kWavesOfAttention, 2) void cache_attention_rows_kernel(CacheAttentionPlan p) {
     typedef AttentionWave<T, NL, RT, CUT> Wave;

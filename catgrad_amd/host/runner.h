@@ -33,7 +33,7 @@ int cgm_set_config(cgm_session *s, int arch, size_t hidden_size, size_t num_hidd
  * CG_BF16 for matrices held and multiplied at bfloat16 precision (Loretar).  Ends every request in progress.
  * Llama and Qwen3: with "kv_cache": "f8" keys and values are held as 8-bit codes, a fourth of the memory, with a scale for each 64
  * positions of a head (heads of 16, 32, .. 256 channels; the codes' rounding is part of the answers), and "rope_scaling" is followed
- * ("linear", "llama3", "yarn" without "mscale" and with "truncate"; without "kv_cache" it is not read).  A request begins with room for 64 positions, or for what
+ * ("linear", "llama3", "yarn"; "mscale" and "truncate": false are refused; without "kv_cache" it is not read).  A request begins with room for 64 positions, or for what
  * its first steps say in max_positions, and grows.  A step writes into the caches where they are: one that fails ends its
  * request, whose next steps are refused until `end`. */
 int cgm_load_config(cgm_session *s, const char *json, int weights_dtype);
