@@ -15,9 +15,11 @@
 // in [2^7, 2^8), and is one 16-bit float a value, or with 32-bit inputs the sum of two (2^-23 of the row's largest; 16-bit inputs are
 // exact but where they lie 2^22 below it).  Bfloat16 queries of more than 64 channels are two codes instead, the nearest and the nearest to what is left, together exact but
 // where they lie 2^14 below the row's largest (there to 2^-22 of it): then the instruction takes the keys' codes as they are (v_mfma_scale_f32_16x16x128_f8f6f4, at twice the rate, so that the two cost
-// what one 16-bit float does, without the widening of keys: four prompts of 2048 tokens of 16 heads of 128, 84 us against 89).  A block's scale multiplies the scores in 32 bits.  Weights are exp2(score - m + 8) <= 2^15
-// with m the running maximum, which moves only where a score is 7 or more above it (most tiles move none: then nothing is
-// rescaled), as one 16-bit float (2^-12) or two (2^-23), and so is their sum, by the same instruction from ones.  Either way a weight is off by up to
+// what one 16-bit float does, without the widening of keys: four prompts of 2048 tokens of 16 heads of 128, 84 us against 89).  A block's scale multiplies the scores in 32 bits.  Weights are exp2(score - m) <= 2^15
+// with m the running maximum less 8, which moves only where a score is 15 or more above it (most tiles move none: then nothing is
+// rescaled).  A score is a product whose difference from m is rounded once; behind a maximum beyond 2^20 the product is rounded first, as the maximum is, so that no score seems to lie above
+// its own maximum; where 8 is less than half a step of the scores, m is the maximum itself.  Weights are held
+// as one 16-bit float (2^-12) or two (2^-23), and so is their sum, by the same instruction from ones.  Either way a weight is off by up to
 // 2^-33 of its row's largest, and may be zero below that.
 // Totals are in units of a scale 2^unit.  Where many rows have 16-bit results and all value blocks that a workgroup's rows see have scales within
 // 2^15 of each other (they are looked over in front: ScaleRange), the unit is the largest of them, codes are widened times their scale in it, which is exact, and
@@ -50,6 +52,7 @@ typedef short short2v __attribute__((ext_vector_type(2)));
 constexpr uint32_t kTile = 64;           // positions of a wave's tile
 constexpr uint32_t kWavesOfAttention = 4;
 constexpr float kNoMaximum = -3.0e38f;   // of a row that has seen nothing
+constexpr float kFar = 0x1p20f;          // scores below are rounded by less than 2^-4
 constexpr uint32_t kMostTiles = 65536;   // that the instruction adds to totals itself
 constexpr int kExact = 15; // a code times 2^-15 is exact as a 16-bit float (whole multiples of 2^-9, 2^-24)
 // The fewest tiles worth a part of their own: of a token behind 8000 12.9 us, with eight 14.4; a prompt of 1024 tokens of nine heads 23 us, with eight 34.
@@ -123,7 +126,8 @@ template <class T, int NL, int RT, bool CUT = false> struct AttentionWave {
     // Totals: sums of weight * value in units of 2^unit.  sums: of the weights, by the same instruction from ones; the first counts.
     float4v total[RT][NV];
     float4v sums[RT];
-    float maximum[RT];
+    float maximum[RT];    // less 8: see the top
+    bool rounded = false; // scores are rounded in front of their difference from it
     int unit = kLowestScale;
     // of the tile at hand
     float4v score[RT][4];
@@ -332,23 +336,34 @@ template <class T, int NL, int RT, bool CUT = false> struct AttentionWave {
                 for (int i = 0; i < 16; i++) m = fmaxf(m, score[rt][i / 4][i % 4]);
             }
             largest[rt] = m == -INFINITY ? m : m * factor[rt]; // (a block that nobody has begun may have any scale: a negative one would make this infinite)
-            moves = moves || largest[rt] > maximum[rt] + 7.0f;
+            moves = moves || largest[rt] - maximum[rt] > 15.0f;
         }
         if (__any(moves)) {
+            bool far = false;
 #pragma unroll
             for (int rt = 0; rt < RT; rt++) {
-                const float m = fmaxf(maximum[rt], quads_max(largest[rt])), down = __builtin_amdgcn_exp2f(maximum[rt] - m);
+                const float top = quads_max(largest[rt]), below = top - 8.0f, m = fmaxf(maximum[rt], top - below > 8.0f ? top : below);
+                const float down = __builtin_amdgcn_exp2f(maximum[rt] - m);
                 maximum[rt] = m;
+                far = far || (fabsf(m) > kFar && m > kNoMaximum);
                 sums[rt][0] *= down;
 #pragma unroll
                 for (int v = 0; v < NV; v++) total[rt][v] *= down;
             }
+            rounded = __any(far) || rounded;
+        }
+        if (rounded) {
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++) {
+#pragma unroll
+                for (int i = 0; i < 16; i++) score[rt][i / 4][i % 4] *= factor[rt];
+                factor[rt] = 1.0f;
+            }
         }
 #pragma unroll
         for (int rt = 0; rt < RT; rt++) {
-            const float above = 8.0f - maximum[rt];
 #pragma unroll
-            for (int i = 0; i < 16; i++) score[rt][i / 4][i % 4] = __builtin_amdgcn_exp2f(fmaf(score[rt][i / 4][i % 4], factor[rt], above));
+            for (int i = 0; i < 16; i++) score[rt][i / 4][i % 4] = __builtin_amdgcn_exp2f(fmaf(score[rt][i / 4][i % 4], factor[rt], -maximum[rt]));
             if (masked) {
 #pragma unroll
                 for (int i = 0; i < 16; i++) score[rt][i / 4][i % 4] = sees(rt, i) ? score[rt][i / 4][i % 4] : 0.0f;

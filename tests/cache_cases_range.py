@@ -120,3 +120,34 @@ def run_rows_apart(lib, device, form, block):
         want, size, terms = R.attend(x[s], held + s, keys, values, D ** -0.5, 0)
         tol = 2 * (TERMS[dtype] * terms + 2.0 ** -20 + WEIGHT[dtype]) * size + HALF[dtype] * np.abs(want) + 16 * 2.0 ** -157 * 2.0 ** -7 * large
         off_by(y[s], want, tol, f"{form} {block} row {s}")
+
+
+def run_large_scores(lib, device, form, block):
+    """Scores far beyond 2^22, where a 32-bit float has no room for what an exponent is told from it by: keys that are the same weigh the same, and one that is
+    larger than all others has all of the weight.  Weights then are equal, or one and zero: only the sums' and the results' roundings are left."""
+    dtype, S, H, D, V, _ = FORMS[form]
+    rng = np.random.default_rng(block)
+    T = 150
+    v = rng.uniform(0.5, 1.0, (1, T, V))
+    for power in range(18, 61, 1) if dtype != "f16" else range(18, 31):
+        for sign in (1.0, -1.0):
+            size = 1.3 * 2.0 ** (power / 2)
+            q, k = np.full((1, S, H * D), size / D ** 0.25), np.full((1, T, D), sign * size / D ** 0.25)
+            for outlier in (False, True):
+                if outlier:
+                    k[:, 70] = 2.0 * np.abs(k[:, 70])
+                cache = Cache(device, 1, 1, D, V, 192 if block < 128 else 256, block)
+                append(lib, device, cache, "f32", [0], [T], k, v)
+                rq, out = Rows(q, dtype, device), Rows(np.zeros((1, S, H * V)), dtype, device)
+                h, c = lengths(device, [T - S], [S])
+                a = A.CacheAttentionRows(A.TokenBatch(1, S, 0, h.data_ptr(), c.data_ptr()), TYPES[dtype][1], rq.rows.data_ptr(), out.rows.data_ptr(), rq.pitch, out.pitch, H,
+                                         cache.struct(), D ** -0.5, 0, None, 0)
+                need = C.c_size_t()
+                check(lib, lib.cg_cache_attention_workspace(a, need))
+                assert need.value == 0  # (so few positions are not cut)
+                check(lib, lib.cg_cache_attention_noalloc(0, a, stream_of(device)))
+                x, y = f64(rq.rows).reshape(S, H, D), f64(out.rows).reshape(S, H, V)
+                keys, values = (t.x for t in cache.heads[0][0])
+                for s in range(S):
+                    want, size_of, _ = R.attend(x[s], T - S + s, keys, values, D ** -0.5, 0)
+                    off_by(y[s], want, 2.0 ** -20 * size_of + HALF[dtype] * np.abs(want), f"2^{power} {sign} {outlier} {form} {block} row {s}")

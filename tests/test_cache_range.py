@@ -27,3 +27,8 @@ def test_large(oracle, form, block):
 @pytest.mark.parametrize("form,block", [("few_f32", 16), ("few_bf16_20_rows", 64)])
 def test_rows_apart(oracle, form, block):
     E.run_rows_apart(oracle._lib, "cpu", form, block)
+
+
+@pytest.mark.parametrize("form,block", [("few_f32", 16), ("few_f16", 64)])
+def test_large_scores(oracle, form, block):
+    E.run_large_scores(oracle._lib, "cpu", form, block)

@@ -39,3 +39,9 @@ def test_large_in_parts(hip, form, positions):
 @pytest.mark.parametrize("form", [f for f in E.FORMS if "_f16" not in f])
 def test_rows_apart(hip, form, block):
     E.run_rows_apart(hip._lib, "cuda", form, block)
+
+
+@pytest.mark.parametrize("block", [16, 64])
+@pytest.mark.parametrize("form", list(E.FORMS))
+def test_large_scores(hip, form, block):
+    E.run_large_scores(hip._lib, "cuda", form, block)
