@@ -406,6 +406,21 @@ template <class T, int NL, int RT, bool CUT = false> struct AttentionWave {
                 clean();
             }
         }
+        int e = scale_exponent(vs), largest_e = 0, smallest_e = 0; // of the lane's value block; of the tile
+        if constexpr (!DIRECT) {
+            if (p.cache.block_log2 < 6) {
+                const bool seen = mine + 15 >= any_from && mine <= any_to; // (a block that no row sees counts for nothing: its scale may be anything)
+                const int none = -1000;
+                largest_e = quads_max(seen ? e : none);
+                smallest_e = -quads_max(seen ? -e : none);
+                if (largest_e == none) largest_e = smallest_e = kLowestScale;
+                e = seen ? e : largest_e;
+            } else {
+                largest_e = smallest_e = e;
+            }
+            largest_e = __builtin_amdgcn_readfirstlane(largest_e);
+            smallest_e = __builtin_amdgcn_readfirstlane(smallest_e);
+        }
         half8v w[RT][kPieces][2];
         const half8v ones = {1, 1, 1, 1, 1, 1, 1, 1};
 #pragma unroll
@@ -450,24 +465,10 @@ template <class T, int NL, int RT, bool CUT = false> struct AttentionWave {
                 }
             }
         };
-        int e = scale_exponent(vs); // of the lane's block
         if constexpr (DIRECT) {
             asm volatile("" ::: "memory");
             add(power_of_two(min(max(e - unit, -kExact), 0)), 1.0f); // (a block that no row sees may have any scale: its weights are zero)
         } else {
-            int largest_e, smallest_e; // of the tile
-            if (p.cache.block_log2 < 6) {
-                const bool seen = mine + 15 >= any_from && mine <= any_to; // (a block that no row sees counts for nothing: its scale may be anything)
-                const int none = -1000;
-                largest_e = quads_max(seen ? e : none);
-                smallest_e = -quads_max(seen ? -e : none);
-                if (largest_e == none) largest_e = smallest_e = kLowestScale;
-                e = seen ? e : largest_e;
-            } else {
-                largest_e = smallest_e = e;
-            }
-            largest_e = __builtin_amdgcn_readfirstlane(largest_e);
-            smallest_e = __builtin_amdgcn_readfirstlane(smallest_e);
             const int passes = largest_e - smallest_e > kExact ? 4 : 1; // (the same for all lanes of a wave)
             for (int pass = 0; pass < passes; pass++) {
                 asm volatile("" ::: "memory");
@@ -753,7 +754,7 @@ template <class T, int NL, int RT, bool CUT = false> __global__ __launch_bounds_
         to = w.any_to < 0 ? 0 : (uint32_t)w.any_to / kTile + 1;
     }
     const bool near = few_tiles && scales.near(&w.unit);
-    auto walk = [&](auto direct) __attribute__((always_inline)) {
+    auto walk = [&](auto direct) {
         for (uint32_t t = my.tile; t < my.end_tile; t++) {
             const uint32_t place = (t - my.tile) & 1;
             asm volatile("" ::: "memory");
